@@ -25,6 +25,10 @@ ACT_GELU_ERF, ACT_LEAKY_RELU, ACT_ELU = 4, 5, 6
 BIAS_NE0, BIAS_NE1 = 0, 1
 # error-word bits of cbx_embed_gather_add
 EFLAG_TOKEN_OOB, EFLAG_POS_OOB = 0x1, 0x2
+# error-word bits of the paged entry points and cbx_token_logprobs
+EFLAG_NO_PAGE, EFLAG_PAGE_OOB, EFLAG_LENGTH = 0x4, 0x8, 0x10
+# limits of the paged entry points and cbx_token_logprobs
+PAGED_MAX_REQS, LOGPROBS_MAX_TOP = 8192, 32
 # bits of the library's device error word (cbx_device_errors)
 DEVERR_WAIT_TIMEOUT = 0x1
 
@@ -71,6 +75,17 @@ SIGNATURES = {
     "cbx_hann_window": ([_i32, _vp], ctypes.c_int),
     "cbx_qkv_kv_append": ([_vp, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp,
                            _vp, _vp], ctypes.c_int),
+    "cbx_paged_plan": ([_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                        _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
+    "cbx_qkv_kv_append_paged": ([_vp, _i32, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32,
+                                 _i64, _i64, _i64, _vp, _vp, _vp], ctypes.c_int),
+    "cbx_paged_decode_attention": ([_vp, _i32, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64,
+                                    _i64, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp,
+                                    _i64, _vp, _vp], ctypes.c_int),
+    "cbx_paged_decode_attention_workspace": ([_i64, _i64, _i64, _i64, _i64, _i64, _i32],
+                                             ctypes.c_int64),
+    "cbx_token_logprobs": ([_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                            _vp], ctypes.c_int),
 }
 
 _lock = threading.Lock()

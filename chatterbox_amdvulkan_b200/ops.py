@@ -17,6 +17,10 @@ helpers they replace:
   sum3_scale         hift_vocoder.cpp:733-739 (ResBlock average)
   sinusoidal_pos_emb cfm_decoder.cpp:49-62 (batched, on the device)
   snake              hift_vocoder.cpp:64-73
+  qkv_kv_append_paged  t3.cpp:465-489 on a paged KV cache
+  paged_plan, paged_decode_attention, token_logprobs: the rest of a paged decode
+                     step (block tables and slots, attention, the answer's log
+                     probabilities); the engine decodes one slab per stream
 
 There is no CPU path: inputs must be CUDA tensors and the shared library must
 be present, otherwise these raise.
@@ -25,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -584,3 +589,264 @@ def qkv_kv_append(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: torch.T
               int(slab_stride), int(max_context), _dev(q, "q", torch.float32),
               _dev(err, "err", torch.int32), _stream(qkv))
     return q, err
+
+
+# ------------------------------------------------------- paged KV cache --
+
+def _paged_cache(cache_k: torch.Tensor, cache_v: torch.Tensor):
+    """(n_pages, page_size, n_kv_heads, head_dim, page_stride) of two caches
+    [n_pages, page_size, n_kv_heads, head_dim]: the last three dimensions dense, the pages a
+    fixed stride apart (so a cache can be one layer of a pool [n_pages, n_layers, 2, ...])."""
+    if cache_k.dim() != 4 or cache_v.shape != cache_k.shape:
+        raise ValueError("cache_k and cache_v must be [n_pages, page_size, n_kv_heads, head_dim] "
+                         f"of one shape, got {tuple(cache_k.shape)} and {tuple(cache_v.shape)}")
+    if cache_k.dtype != cache_v.dtype:
+        raise TypeError("cache_k and cache_v must share a dtype")
+    P, S, Hk, hd = cache_k.shape
+    if cache_k.numel() == 0:
+        raise ValueError(f"the caches are empty: shape {tuple(cache_k.shape)}")
+    strides = cache_k.stride()
+    # the stride of a dimension of one entry means nothing
+    dense = all(n == 1 or s == d for n, s, d in
+                zip((S, Hk, hd), strides[1:], (Hk * hd, hd, 1)))
+    page_stride = strides[0] if P > 1 else S * Hk * hd
+    if not dense or page_stride < S * Hk * hd or (P > 1 and cache_v.stride(0) != page_stride) or \
+            not all(n == 1 or a == b for n, a, b in zip((S, Hk, hd), cache_v.stride()[1:],
+                                                       strides[1:])):
+        raise ValueError("the caches' pages must be dense [page_size, n_kv_heads, head_dim] blocks "
+                         f"and equally far apart, got strides {strides} and {cache_v.stride()}")
+    return P, S, Hk, hd, page_stride
+
+
+def _here(t: torch.Tensor, name: str, dtype=None) -> int:
+    """Address of a CUDA tensor of any strides (the caller checks them)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (libcbx_ops has no CPU path)")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the call runs on "
+                         f"cuda:{torch.cuda.current_device()}: all tensors of a call must "
+                         "share its device")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    return t.data_ptr()
+
+
+def _err_word(err: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    if err is None:
+        return torch.zeros(1, dtype=torch.int32, device=like.device)
+    if err.numel() < 1:
+        raise ValueError("err must hold one int32")
+    return err
+
+
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` returns: the step's rows, then the state after it."""
+    slots: torch.Tensor        # [max_rows] cache slot of each row, -1: none
+    positions: torch.Tensor    # [max_rows]
+    row_reqs: torch.Tensor     # [max_rows] request of each row
+    row_lens: torch.Tensor     # [max_rows] keys a row attends to: position + 1
+    row_start: torch.Tensor    # [n_reqs + 1] first row of each request
+    block_table: torch.Tensor  # [n_reqs, max_blocks]
+    n_blocks: torch.Tensor     # [n_reqs]
+    free_list: torch.Tensor    # [n_pages]
+    n_free: torch.Tensor       # [1]
+    err: torch.Tensor          # [1] device error word (EFLAG_NO_PAGE, _PAGE_OOB, _LENGTH)
+
+
+@_on_tensor_device
+def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torch.Tensor,
+               free_list: torch.Tensor, n_free: torch.Tensor, page_size: int,
+               n_new: torch.Tensor | None = None, max_rows: int | None = None,
+               in_place: bool = False, out=None, err: torch.Tensor | None = None) -> PagedPlan:
+    """Block tables, slots and positions of one step, on the device (see cbx_paged_plan).
+
+    seq_lens: int32 [n_reqs], the tokens each request holds after the step (0: ended or empty);
+    n_new: int32 [n_reqs], how many of them, the last ones, the step writes (None: one for each
+    request that is there); max_rows: rows to lay out (None: n_reqs).  State: block_table int32
+    [n_reqs, max_blocks], n_blocks int32 [n_reqs], free_list int32 [n_pages], n_free int32 [1].
+    With ``in_place`` the state tensors are updated, otherwise new ones are returned; ``out``
+    (the first 9 tensors of an earlier plan of the same sizes) gives the buffers."""
+    if block_table.dim() != 2 or block_table.shape[0] != seq_lens.numel():
+        raise ValueError(f"block_table must be [n_reqs, max_blocks], got {tuple(block_table.shape)} "
+                         f"for {seq_lens.numel()} requests")
+    n_reqs, max_blocks = block_table.shape
+    if n_blocks.numel() != n_reqs or n_free.numel() != 1 or \
+            (n_new is not None and n_new.numel() != n_reqs):
+        raise ValueError("n_blocks and n_new must hold n_reqs entries, n_free one")
+    max_rows = n_reqs if max_rows is None else int(max_rows)
+    if out is not None:
+        if in_place:
+            raise ValueError("out and in_place exclude one another")
+        out = tuple(out)[:9]
+        sizes = [max_rows] * 4 + [n_reqs + 1, n_reqs * max_blocks, n_reqs, free_list.numel(), 1]
+        if [t.numel() for t in out] != sizes:
+            raise ValueError(f"out must hold 9 tensors of {sizes} entries")
+    else:
+        def new(n):
+            return torch.empty(n, dtype=torch.int32, device=seq_lens.device)
+        rows = [new(max_rows) for _ in range(4)] + [new(n_reqs + 1)]
+        state = (block_table, n_blocks, free_list, n_free)
+        out = (*rows, *(state if in_place else map(torch.empty_like, state)))
+    err = _err_word(err, seq_lens)
+    i32 = torch.int32
+    slots, positions, row_reqs, row_lens, row_start, table_o, blocks_o, free_o, n_free_o = (
+        _dev(t, "out", i32) for t in out)
+    _lib.call("cbx_paged_plan", _dev(seq_lens, "seq_lens", i32), _dev(n_new, "n_new", i32), n_reqs,
+              max_blocks, int(page_size), free_list.numel(), _dev(block_table, "block_table", i32),
+              _dev(n_blocks, "n_blocks", i32), _dev(free_list, "free_list", i32),
+              _dev(n_free, "n_free", i32), table_o, blocks_o, free_o, n_free_o, max_rows, slots,
+              positions, row_reqs, row_lens, row_start, _dev(err, "err", i32), _stream(seq_lens))
+    return PagedPlan(*out, err)
+
+
+@_on_tensor_device
+def qkv_kv_append_paged(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: torch.Tensor,
+                        cache_v: torch.Tensor, slots: torch.Tensor,
+                        q_out: torch.Tensor | None = None, err: torch.Tensor | None = None,
+                        with_q: bool = True):
+    """qkv bias add + Q + K / V written into pages (t3.cpp:465-489 on a paged cache).
+
+    qkv: f32 / f16 / bf16 [n_rows, q_dim + 2 kv_dim] (rows may be strided); bias: f32 or None;
+    caches [n_pages, page_size, n_kv_heads, head_dim]; slots: int32 [n_rows], page * page_size +
+    place, -1 skips the row.  Returns (q [n_rows, q_dim] of qkv's dtype or None, err).  The q
+    rows of skipped rows are left as they were in q_out (without q_out: unspecified)."""
+    if qkv.dim() != 2 or (qkv.shape[0] > 0 and qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise ValueError("qkv must be 2-D [n_rows, q_dim + 2 kv_dim] with dense rows, got shape "
+                         f"{tuple(qkv.shape)} strides {qkv.stride()}")
+    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
+    n_rows, width = qkv.shape
+    kv_dim = Hk * hd
+    q_dim = width - 2 * kv_dim
+    if q_dim < 0:
+        raise ValueError(f"qkv's row length {width} is below 2 kv_dim = {2 * kv_dim}")
+    stride = qkv.stride(0) if n_rows > 1 else width
+    if stride < width:
+        raise ValueError(f"qkv's rows overlap: stride {stride} < {width}")
+    if slots.numel() < n_rows:
+        raise ValueError(f"slots has {slots.numel()} entries for {n_rows} rows")
+    if bias is not None and bias.numel() != width:
+        raise ValueError(f"bias has {bias.numel()} entries, expected {width}")
+    if q_out is not None and (q_out.numel() != n_rows * q_dim or q_out.dtype != qkv.dtype):
+        raise ValueError(f"q_out must hold {n_rows} x {q_dim} values of {qkv.dtype}")
+    if q_out is None and with_q:
+        q_out = torch.empty((n_rows, q_dim), dtype=qkv.dtype, device=qkv.device)
+    err = _err_word(err, qkv)
+    _lib.call("cbx_qkv_kv_append_paged", _here(qkv, "qkv"), _cbx_type(qkv), stride,
+              _dev(bias, "bias", torch.float32), n_rows, q_dim, kv_dim,
+              _dev(slots, "slots", torch.int32), _here(cache_k, "cache_k"),
+              _here(cache_v, "cache_v"), _cbx_type(cache_k), P, S, page_stride,
+              _dev(q_out, "q_out"), _dev(err, "err", torch.int32), _stream(qkv))
+    return q_out, err
+
+
+@_on_tensor_device
+def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
+                           block_table: torch.Tensor, seq_lens: torch.Tensor,
+                           row_reqs: torch.Tensor | None = None, scale: float | None = None,
+                           return_lse: bool = False, out: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None,
+                           err: torch.Tensor | None = None):
+    """softmax(scale q K^T) V of one new token per row over a paged cache.
+
+    q: [n_rows, n_heads, head_dim] f32 / f16 / bf16 (rows may be strided); caches [n_pages,
+    page_size, n_kv_heads, head_dim]; block_table: int32 [n_reqs, max_blocks]; seq_lens: int32
+    [n_rows], the keys of each row (0: zeros); row_reqs: int32 [n_rows], each row's request (None:
+    row r is request r); scale: head_dim ** -0.5 by default.  Returns out [n_rows, n_heads,
+    head_dim] of q's dtype, with ``return_lse`` (out, lse f32 [n_rows, n_heads]).  ``workspace``:
+    a byte tensor of ``paged_decode_attention_workspace`` bytes to use instead of a new one."""
+    if q.dim() != 3 or (q.numel() > 0 and not q[0].is_contiguous()):
+        raise ValueError("q must be [n_rows, n_heads, head_dim] with dense rows, got shape "
+                         f"{tuple(q.shape)} strides {q.stride()}")
+    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
+    n_rows, H, qd = q.shape
+    if qd != hd:
+        raise ValueError(f"q's head_dim {qd} is not the caches' {hd}")
+    q_stride = q.stride(0) if n_rows > 1 else H * hd
+    if q_stride < H * hd:
+        raise ValueError(f"q's rows overlap: stride {q_stride}")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [n_reqs, max_blocks], got {tuple(block_table.shape)}")
+    n_reqs, max_blocks = block_table.shape
+    if seq_lens.numel() != n_rows or (row_reqs is not None and row_reqs.numel() != n_rows):
+        raise ValueError(f"seq_lens and row_reqs must hold one entry for each of {n_rows} rows")
+    if row_reqs is None and n_reqs < n_rows:
+        raise ValueError(f"block_table has {n_reqs} rows for {n_rows} rows of q")
+    if out is None:
+        out = torch.empty((n_rows, H, hd), dtype=q.dtype, device=q.device)
+    elif out.numel() != n_rows * H * hd or out.dtype != q.dtype:
+        raise ValueError(f"out must hold {n_rows} x {H} x {hd} values of {q.dtype}")
+    lse = torch.empty((n_rows, H), dtype=torch.float32, device=q.device) if return_lse else None
+    ct = _cbx_type(cache_k)
+    q_ptr = _here(q, "q")
+    need = _workspace_bytes(n_rows, H, Hk, hd, max_blocks, S, ct)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    err = _err_word(err, q)
+    _lib.call("cbx_paged_decode_attention", q_ptr, _cbx_type(q), q_stride,
+              _here(cache_k, "cache_k"), _here(cache_v, "cache_v"), ct, P, S, page_stride,
+              _dev(block_table, "block_table", torch.int32), n_reqs, max_blocks,
+              _dev(row_reqs, "row_reqs", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
+              n_rows, H, Hk, hd, float(hd ** -0.5 if scale is None else scale), _dev(out, "out"),
+              _dev(lse, "lse"), _dev(workspace, "workspace") if need else None,
+              workspace.numel() * workspace.element_size() if need else 0,
+              _dev(err, "err", torch.int32), _stream(q))
+    return (out, lse) if return_lse else out
+
+
+def _workspace_bytes(n_rows, n_heads, n_kv_heads, head_dim, max_blocks, page_size, cache_type):
+    n = _lib.load().cbx_paged_decode_attention_workspace(n_rows, n_heads, n_kv_heads, head_dim,
+                                                         max_blocks, page_size, cache_type)
+    if n < 0:
+        _lib.check("cbx_paged_decode_attention_workspace", int(n))
+    return n
+
+
+def paged_decode_attention_workspace(n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                                     max_blocks: int, page_size: int,
+                                     cache_dtype: torch.dtype = torch.float32) -> int:
+    """Bytes of workspace ``paged_decode_attention`` needs for these sizes on the current device."""
+    return _workspace_bytes(int(n_rows), int(n_heads), int(n_kv_heads), int(head_dim),
+                            int(max_blocks), int(page_size), _TORCH_TO_CBX[cache_dtype])
+
+
+# ------------------------------------------------- token log probabilities --
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns (natural logarithms, f32)."""
+    logprobs: torch.Tensor | None      # [n_rows] of the given tokens
+    entropy: torch.Tensor              # [n_rows]
+    top_ids: torch.Tensor              # [n_rows, top_k] int32
+    top_logprobs: torch.Tensor         # [n_rows, top_k]
+    err: torch.Tensor                  # [1] device error word (EFLAG_TOKEN_OOB)
+
+
+@_on_tensor_device
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top_k: int = 0,
+                   err: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log probabilities of given tokens, entropy and the top_k most probable alternatives.
+
+    logits: f32 / f16 / bf16 [n_rows, vocab] (rows may be strided); tokens: int32 [n_rows] (-1: no
+    token, NaN) or None; ties among the alternatives go to the lowest id."""
+    if logits.dim() != 2 or (logits.shape[0] > 0 and logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be 2-D [n_rows, vocab] with dense rows, got shape "
+                         f"{tuple(logits.shape)} strides {logits.stride()}")
+    n_rows, vocab = logits.shape
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(vocab, _lib.LOGPROBS_MAX_TOP):
+        raise ValueError(f"top_k {top_k} outside [0, min(vocab, {_lib.LOGPROBS_MAX_TOP})]")
+    stride = logits.stride(0) if n_rows > 1 else vocab
+    if stride < vocab:
+        raise ValueError(f"logits' rows overlap: stride {stride} < {vocab}")
+    if tokens is not None and tokens.numel() != n_rows:
+        raise ValueError(f"tokens has {tokens.numel()} entries for {n_rows} rows")
+    dev = logits.device
+    lp = torch.empty(n_rows, dtype=torch.float32, device=dev) if tokens is not None else None
+    entropy = torch.empty(n_rows, dtype=torch.float32, device=dev)
+    ids = torch.empty((n_rows, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((n_rows, top_k), dtype=torch.float32, device=dev)
+    err = _err_word(err, logits)
+    _lib.call("cbx_token_logprobs", _here(logits, "logits"), _cbx_type(logits), stride, n_rows,
+              vocab, _dev(tokens, "tokens", torch.int32), top_k, _dev(lp, "logprobs"),
+              _dev(entropy, "entropy"), _dev(ids, "top_ids"), _dev(top, "top_logprobs"),
+              _dev(err, "err", torch.int32), _stream(logits))
+    return TokenLogprobs(lp, entropy, ids, top, err)

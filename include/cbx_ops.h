@@ -102,6 +102,10 @@ typedef enum cbx_bias_axis {
 /* Bits of the optional device error word of cbx_embed_gather_add. */
 #define CBX_EFLAG_TOKEN_OOB 0x1
 #define CBX_EFLAG_POS_OOB   0x2
+/* Further bits, raised by the paged entry points and cbx_token_logprobs. */
+#define CBX_EFLAG_NO_PAGE   0x4  /* the pool has too few free pages, or a table row too few entries */
+#define CBX_EFLAG_PAGE_OOB  0x8  /* a page, slot or request index outside its range                 */
+#define CBX_EFLAG_LENGTH    0x10 /* a length, count or row total outside its range (clamped)        */
 
 /* Bits of the library's own device error word (see cbx_device_errors). */
 #define CBX_DEVERR_WAIT_TIMEOUT 0x1 /* a bounded wait on a TMA transfer gave up */
@@ -403,6 +407,152 @@ CBX_API int cbx_qkv_kv_append(const float* qkv, int64_t qkv_row_stride, const fl
                               int32_t pos_offset, void* cache_k, void* cache_v, int cache_type,
                               int64_t slab_stride, int64_t max_context, float* q_out,
                               int32_t* err_word, cbx_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * Paged KV cache: the cache memory of one layer is n_pages pages of page_size
+ * tokens, cache[page][token in page][kv_dim].  A request owns the pages that
+ * its row of the block table names; token p of request b lives in slot
+ *   table[b][p / page_size] * page_size + p % page_size.
+ * The engine keeps one slab of max_context rows per stream
+ * (chatterbox-cpp/src/t3.cpp:238-262); pages let requests of unequal length
+ * share the memory.  The pages of a request are shared by all layers.
+ *
+ * cbx_paged_plan: one step's block tables, slots and positions, built on the
+ * device from the requests' lengths.
+ *   seq_lens[b]  tokens request b holds after the step (0: it has ended, or
+ *                its place in the batch is empty)
+ *   n_new[b]     how many of them, the last ones, the step writes (NULL: one
+ *                for each request with a length above 0)
+ * State (in -> out; each out pointer may equal its in pointer, or must not
+ * overlap any input):
+ *   table    [n_reqs][max_blocks] page ids, -1 behind the first n_blocks[b]
+ *   n_blocks [n_reqs]             pages that request b owns
+ *   free     [n_pages]            a stack of free page ids; entries at and
+ *                                 behind n_free are not part of it
+ *   n_free   [1]
+ * With need[b] = ceil(seq_lens[b] / page_size): pages that a request no longer
+ * needs go back on the stack (in the order of b, then of the block), then the
+ * missing ones are popped (in the same order).  So a request that ended, or
+ * was cut back, returns its pages in this call, and they can be given out
+ * again in it.
+ * Per row t < max_rows of the step (requests in order, tokens in order):
+ *   slots[t], positions[t], row_reqs[t] = b, row_lens[t] = positions[t] + 1
+ * and row_start [n_reqs + 1], the first row of each request.  Rows behind the
+ * last token: slot -1, position 0, request 0, length 0 (they are skipped by
+ * cbx_qkv_kv_append_paged and give zeros in cbx_paged_decode_attention).
+ * row_reqs / row_lens / row_start may be NULL.
+ * Device errors (ORed into *err_word): a pool or table row with too few pages
+ * (CBX_EFLAG_NO_PAGE: the request gets what is left, tokens without a page get
+ * slot -1); a negative length, n_new outside [0, seq_lens], a length above
+ * max_blocks * page_size, more rows than max_rows, state counts outside their
+ * range (CBX_EFLAG_LENGTH: clamped, rows behind max_rows dropped); a page id
+ * outside [0, n_pages) (CBX_EFLAG_PAGE_OOB, slot -1).
+ * n_reqs <= CBX_PAGED_MAX_REQS; n_pages * page_size, n_reqs * max_blocks and
+ * max_rows below 2^31.  Integer results, the same in every run.
+ * ------------------------------------------------------------------------- */
+#define CBX_PAGED_MAX_REQS 8192
+CBX_API int cbx_paged_plan(const int32_t* seq_lens, const int32_t* n_new, int64_t n_reqs,
+                           int64_t max_blocks, int64_t page_size, int64_t n_pages,
+                           const int32_t* table_in, const int32_t* n_blocks_in,
+                           const int32_t* free_in, const int32_t* n_free_in, int32_t* table_out,
+                           int32_t* n_blocks_out, int32_t* free_out, int32_t* n_free_out,
+                           int64_t max_rows, int32_t* slots, int32_t* positions,
+                           int32_t* row_reqs, int32_t* row_lens, int32_t* row_start,
+                           int32_t* err_word, cbx_stream_t stream);
+
+/* The QKV epilogue (t3.cpp:465-489, as cbx_qkv_kv_append) with K and V written
+ * into pages, grouped heads included: for each row r with slot s = slots[r],
+ *   t = qkv[r][i] + qkv_bias[i]                  (f32, one add)
+ *   q_out[r][i] = (Tq)t                          0 <= i < q_dim
+ *   cache_k[s / page_size * page_stride + s % page_size * kv_dim + i] = (Tc)t
+ *   cache_v[...] = (Tc)t                         the next kv_dim, and the last
+ * qkv_type (and that of q_out, Tq) and cache_type: any of F32 / F16 / BF16; one
+ * rounding each.  qkv rows are qkv_row_stride elements apart (0 = q_dim +
+ * 2 kv_dim); page_stride (0 = page_size * kv_dim) is in elements, so that a
+ * cache can be a view of a pool that holds all layers.  qkv_bias f32 or NULL;
+ * q_out may be NULL.  A row with slot -1 is skipped, its q_out row left as it
+ * was; any other slot outside [0, n_pages * page_size) writes no cache row and
+ * ORs CBX_EFLAG_PAGE_OOB into *err_word (its q_out row is written).  Two rows
+ * with one slot leave either's values there.  q_out and the caches must not
+ * overlap the inputs. */
+CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_row_stride,
+                                    const float* qkv_bias, int64_t n_rows, int64_t q_dim,
+                                    int64_t kv_dim, const int32_t* slots, void* cache_k,
+                                    void* cache_v, int cache_type, int64_t n_pages,
+                                    int64_t page_size, int64_t page_stride, void* q_out,
+                                    int32_t* err_word, cbx_stream_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * Attention of one new token per row over the paged cache (what the engine's
+ * graph computes for one query between t3.cpp:489 and :528).  For row r of
+ * request b = row_reqs ? row_reqs[r] : r, query head h and its kv head
+ * g = h / (n_heads / n_kv_heads), over the keys j < seq_lens[r]:
+ *   s_j = scale * sum_i q[r][h][i] * K[j][g][i]
+ *   out[r][h] = sum_j e^(s_j - m) V[j][g] / sum_j e^(s_j - m),  m = max_j s_j
+ *   lse[r][h] = m + ln sum_j e^(s_j - m)                        (natural log)
+ * q, out: [n_rows][n_heads][head_dim] of q_type, rows q_row_stride elements
+ * apart (0 = dense; out is dense); caches as in cbx_qkv_kv_append_paged with
+ * kv_dim = n_kv_heads * head_dim, of cache_type; table [n_reqs][max_blocks].
+ * q_type and cache_type: any of F32 / F16 / BF16.  Products, softmax and sums
+ * are f32; out is rounded once.  Several rows may name one request (the tokens
+ * of a prefill chunk or of a speculated continuation, each with its length).
+ * A row of length 0 gives zeros and lse -inf.  lse (f32 [n_rows][n_heads]) may
+ * be NULL.  Keys at and behind the length are not read, whatever the memory
+ * holds.  Keys whose table entry is outside [0, n_pages) are left out of the
+ * sums and raise CBX_EFLAG_PAGE_OOB, a row_reqs entry outside [0, n_reqs) does
+ * too (the row counts as empty); a length above max_blocks * page_size or below
+ * 0 is clamped and raises CBX_EFLAG_LENGTH.
+ * n_rows <= 65535; head_dim: a multiple of 8, at most 256; caches 16-byte aligned, page_stride a
+ * multiple of kv_dim and the cache at most 2^31 - 1 rows of kv_dim long
+ * (n_pages * page_stride / kv_dim).  out and lse must not overlap the inputs.
+ * workspace: device memory of cbx_paged_decode_attention_workspace(...) bytes,
+ * 16-byte aligned, for the partial results of a call that is split over the
+ * keys (0 bytes: it may be NULL).  Its contents need no preparation and mean
+ * nothing after the call; calls that may run at the same time need one each.
+ * The same inputs give the same bits.
+ * ------------------------------------------------------------------------- */
+CBX_API int cbx_paged_decode_attention(const void* q, int q_type, int64_t q_row_stride,
+                                       const void* cache_k, const void* cache_v, int cache_type,
+                                       int64_t n_pages, int64_t page_size, int64_t page_stride,
+                                       const int32_t* table, int64_t n_reqs, int64_t max_blocks,
+                                       const int32_t* row_reqs, const int32_t* seq_lens,
+                                       int64_t n_rows, int64_t n_heads, int64_t n_kv_heads,
+                                       int64_t head_dim, float scale, void* out, float* lse,
+                                       void* workspace, int64_t workspace_bytes,
+                                       int32_t* err_word, cbx_stream_t stream);
+
+/* host: bytes of workspace that cbx_paged_decode_attention needs for these
+ * sizes on the current device (0 or more; negative cbx_status on bad sizes). */
+CBX_API int64_t cbx_paged_decode_attention_workspace(int64_t n_rows, int64_t n_heads,
+                                                     int64_t n_kv_heads, int64_t head_dim,
+                                                     int64_t max_blocks, int64_t page_size,
+                                                     int cache_type);
+
+/* ------------------------------------------------------------------------- *
+ * Log probabilities of given tokens under logits x (the rows that the engine
+ * reads back at t3.cpp:612-614), with the entropy and the most probable
+ * alternatives:
+ *   lse = m + ln S,  m = max_j x_j,  S = sum_j e^(x_j - m)
+ *   logprob[r]  = x[r][tokens[r]] - lse
+ *   entropy[r]  = ln S - sum_j (x_j - m) e^(x_j - m) / S              (nats)
+ *   top_ids[r][i], top_logprobs[r][i], i < top_k: the largest x_j - lse in
+ *   falling order, equal ones by rising j
+ * logits: [n_rows] rows of vocab elements, row_stride elements apart (0 =
+ * vocab), of `type` F32 / F16 / BF16; sums in f32; all outputs f32 / int32.
+ * 0 <= top_k <= min(vocab, CBX_LOGPROBS_MAX_TOP).  tokens and logprob may both
+ * be NULL, entropy may be NULL, top_ids / top_logprobs are needed for
+ * top_k > 0 only.  A logit of -inf is a token of probability 0.  A row with a
+ * NaN, a +inf, or nothing but -inf has no distribution: its values are NaN,
+ * its top_ids still the order of the logits (NaN above all, by rising j).  A
+ * token outside [0, vocab) gives logprob NaN and ORs CBX_EFLAG_TOKEN_OOB into
+ * *err_word; -1 (a row without a token) gives NaN and raises nothing.
+ * Outputs must not overlap the inputs.  The same inputs give the same bits.
+ * ------------------------------------------------------------------------- */
+#define CBX_LOGPROBS_MAX_TOP 32
+CBX_API int cbx_token_logprobs(const void* logits, int type, int64_t row_stride, int64_t n_rows,
+                               int64_t vocab, const int32_t* tokens, int64_t top_k,
+                               float* logprob, float* entropy, int32_t* top_ids,
+                               float* top_logprobs, int32_t* err_word, cbx_stream_t stream);
 
 /* ------------------------------------------------------------------------- *
  * HiFT host DSP either side of the Snake stack, on the device.
