@@ -2,27 +2,37 @@
 // probable alternatives, from rows of logits (what the engine reads back to
 // the host at chatterbox-cpp/src/t3.cpp:612-614).
 //
-// With d_j = x_j - m, e_j = e^d_j, S = sum e_j, T = sum e_j d_j:
-//   logprob = d_tok - ln S,   entropy = ln S - T / S.
-// d is at most 0, so nothing overflows, and the entropy has no large terms that
-// cancel.  One pass holds (m, S, T) per thread; a larger maximum m' turns T
-// into c (T + S (m - m')) and S into c S, c = e^(m - m').  Two such states join
-// by the same rule.  d is formed by a subtraction, not as x log2 e - m log2 e in
-// one FMA: the rounding of m log2 e would differ from thread to thread, and
-// logits at the type's lowest value would overflow.
+// With R a whole number near max_j x_j log2 e, d_j = x_j log2 e - R (one FMA),
+// S = sum 2^d_j and T = sum 2^d_j d_j:
+//   entropy = (log2 S - T / S) ln 2,
+//   logprob = x_tok - m - (log2 S - d_max) ln 2,  m the largest logit.
+// No d is much above kSlack, so nothing overflows, and the entropy has no large
+// terms that cancel.  One pass holds (R, S, T) per thread;
+// a larger R' turns T into c (T + S (R - R')) and S into c S, c = 2^(R - R').
+// R is a whole number, so that R, every R - R' and the powers are exact: the
+// states of all threads refer to the same logits (log2 e max x, rounded in each
+// thread, would not).  Logits above 1e37 in magnitude would overflow in
+// x log2 e; a row whose largest is one of them (all of it masked by the type's
+// lowest value, say) is summed again with d = x - m.
 //
-// The order of the alternatives is that of one 64-bit number per element,
-// (x as an ordered integer, then the complement of j), so ties fall to the
-// lowest index and no two elements are equal.
+// Alternatives.  Each thread keeps the largest logit of every segment of its
+// elements.  The threads form 32 groups; the k-th largest of the 32 group
+// maxima, tau, is at most the k-th largest logit (k groups hold one at or above
+// it), so only segments whose largest reaches tau are read again, and their
+// elements at or above tau, a few dozen, are ranked by counting.  The order is
+// that of one 64-bit number per element (x as an ordered integer, then the
+// complement of its index), so ties fall to the lowest index and no two
+// elements are equal.  A row with more candidates than the list holds (a mask
+// that leaves fewer than k, long runs of ties) or without a distribution takes
+// its maxima one after the other instead.
 //
-// Bound by HBM at many rows (each logit is read once); by latency at one row.
+// Bound by HBM at many rows (each logit is read once), by latency at few: NT
+// threads share a row, from a warp each (no barriers; the work per row outside
+// the loop is that of one warp) to a CTA of 512.
 #include "cbx_common.cuh"
 
 namespace cbx {
 namespace {
-
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 
 struct LogprobArgs {
     const void* x;
@@ -38,44 +48,8 @@ struct LogprobArgs {
     int32_t* err;
 };
 
-struct Stat {
-    float m, s, t;  // maximum; sums relative to it
-};
-
-// Differences below this give e = 0; the bound keeps 0 * d from being a NaN.
-constexpr float kLeast = -1e4f;
-
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float m = fmaxf(a.m, b.m);
-    // a state that has seen nothing above -inf has s = t = 0
-    const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - m, kLeast);
-    const float db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - m, kLeast);
-    const float ca = ex2_approx(da * kLog2e), cb = ex2_approx(db * kLog2e);
-    return {m, ca * a.s + cb * b.s, ca * fmaf(a.s, da, a.t) + cb * fmaf(b.s, db, b.t)};
-}
-
-// Adds N elements.  +inf and NaN make s a NaN.
-template <int N>
-__device__ __forceinline__ void add(Stat& st, const float (&f)[N]) {
-    float b = f[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) b = fmaxf(b, f[i]);
-    if (b > st.m) {
-        const float d = st.m == -INFINITY ? 0.0f : fmaxf(st.m - b, kLeast);
-        const float c = ex2_approx(d * kLog2e);
-        st.t = c * fmaf(st.s, d, st.t);
-        st.s *= c;
-        st.m = b;
-    }
-    const float ref = st.m == -INFINITY ? 0.0f : st.m;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float d = f[i] - ref;
-        const float e = ex2_approx(d * kLog2e);
-        st.s += e;
-        st.t = fmaf(e, fmaxf(d, kLeast), st.t);
-    }
-}
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLeast = -1e4f; // 2^d = 0 far above it; keeps 0 * d from being a NaN
 
 // x as an integer that orders like it; -0 as +0, NaN above +inf.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -86,112 +60,466 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ unsigned long long key_of(float x, int j) {
     return (unsigned long long)ordered(x) << 32 | (uint32_t)~j;
 }
+__device__ __forceinline__ float value_of(unsigned long long key) {  // of a key that is no NaN's
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
 __device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsigned long long b) {
     return a > b ? a : b;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_token_logprobs(LogprobArgs a) {
-    constexpr int EV = Vec<T>::n;
-    __shared__ Stat s_stat[kWarps];
-    __shared__ unsigned long long s_key[kWarps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int V = a.vocab;
-    grid_dep_wait();
-    grid_dep_launch();
-    for (int64_t r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
-        const T* x = static_cast<const T*>(a.x) + r * a.stride;
-        // elements before the first 16-byte boundary, whole vectors, the rest
-        int head = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
-        if (head > V) head = V;
-        const int nv = (V - head) / EV, tail = head + nv * EV;
-        Stat st = {-INFINITY, 0.0f, 0.0f};
-        unsigned long long best = 0;
-        auto one = [&](int j) {
-            const float f[1] = {to_f(x[j])};
-            add(st, f);
-            best = max_key(best, key_of(f[0], j));
-        };
-        if (tid < head) one(tid);
-        for (int i = tid; i < nv; i += kThreads) {
-            float f[EV];
-            ldv<T, EV>(x + head + (int64_t)i * EV, f);
-            add(st, f);
+// The reference for a maximum m (any m, NaN aside): m log2 e to the nearest
+// whole number, by the shift of 1.5 * 2^23 (beyond 2^22 it stays near m log2 e,
+// where every float is whole).
+constexpr float kHuge = 1e37f;
+__device__ __forceinline__ float reference_of(float m) {
+    constexpr float kShift = 12582912.0f;
+    const float v = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
+    return __fsub_rn(__fadd_rn(v, kShift), kShift);
+}
+
+// The reference and the two sums relative to it, two halves each.
+struct Stat {
+    float r;
+    float2 s, t;
+    __device__ __forceinline__ void raise(float to) {
+        const float d = fmaxf(r - to, kLeast), c = ex2_approx(d);
+        t = __fmul2_rn(pair(c), __ffma2_rn(s, pair(d), t));
+        s = __fmul2_rn(pair(c), s);
+        r = to;
+    }
+};
+
+// A maximum may lie this far above the reference: 2^d is far from overflow, and
+// T gains no larger terms than log2 S has, so the threads of a warp seldom
+// leave their common path to raise it after their first values.
+constexpr float kSlack = 8.0f;
+
+// Adds N values (N even) whose maximum is b.  NaN and +inf make s a NaN or inf.
+template <int N>
+__device__ __forceinline__ void add(Stat& st, const float2 (&f)[N / 2], float b) {
+    const float to = reference_of(b);
+    if (to > st.r + kSlack) st.raise(to);
+    const float2 ref = pair(-st.r);
 #pragma unroll
-            for (int e = 0; e < EV; ++e) best = max_key(best, key_of(f[e], head + i * EV + e));
-        }
-        if (tid < V - tail) one(tail + tid);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            Stat b = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                      __shfl_xor_sync(0xffffffffu, st.t, o)};
-            st = lane & o ? join(b, st) : join(st, b);
-        }
-        if (lane == 0) s_stat[warp] = st;
-        __syncthreads();
-        st = s_stat[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) st = join(st, s_stat[w]);
-        const float log_s = logf(st.s);
-        const bool bad = st.m == -INFINITY || st.s != st.s;
-        if (tid == 0) {
-            if (a.entropy) a.entropy[r] = bad ? NAN : log_s - st.t / st.s;
-            if (a.logprob) {
-                const int tok = a.tokens[r];
-                float lp = NAN;
-                if (tok >= 0 && tok < V) {
-                    if (!bad) lp = (to_f(x[tok]) - st.m) - log_s;
-                } else if (tok != -1) {
-                    atomicOr(a.err, CBX_EFLAG_TOKEN_OOB);
-                }
-                a.logprob[r] = lp;
-            }
-        }
-        // The largest, then the largest below it, ...
-        for (int k = 0; k < a.top_k; ++k) {
-            unsigned long long b = best;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) b = max_key(b, __shfl_xor_sync(0xffffffffu, b, o));
-            if (lane == 0) s_key[warp] = b;
-            __syncthreads();
-            b = s_key[0];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) b = max_key(b, s_key[w]);
-            const int j = (int)~(uint32_t)b;
-            if (tid == 0) {
-                a.top_ids[r * a.top_k + k] = j;
-                a.top_logprobs[r * a.top_k + k] = bad ? NAN : (to_f(x[j]) - st.m) - log_s;
-            }
-            if (best == b && k + 1 < a.top_k) {  // its owner looks for its next one
-                best = 0;
-                auto next = [&](int i) {
-                    const unsigned long long c = key_of(to_f(x[i]), i);
-                    if (c < b) best = max_key(best, c);
-                };
-                if (tid < head) next(tid);
-                for (int i = tid; i < nv; i += kThreads) {
-                    float f[EV];
-                    ldv<T, EV>(x + head + (int64_t)i * EV, f);
-#pragma unroll
-                    for (int e = 0; e < EV; ++e) {
-                        const unsigned long long c = key_of(f[e], head + i * EV + e);
-                        if (c < b) best = max_key(best, c);
-                    }
-                }
-                if (tid < V - tail) next(tail + tid);
-            }
-            __syncthreads();
-        }
-        __syncthreads();
+    for (int i = 0; i < N / 2; ++i) {
+        const float2 d = __ffma2_rn(f[i], pair(kLog2e), ref);
+        const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        st.s = __fadd2_rn(st.s, e);
+        st.t = __ffma2_rn(e, make_float2(fmaxf(d.x, kLeast), fmaxf(d.y, kLeast)), st.t);
     }
 }
 
+// A row of logits: scalars up to the first 16-byte boundary, whole vectors,
+// scalars behind them.  Thread tid owns scalar tid of either end and the
+// vectors tid, tid + NT, ...
+template <typename T>
+struct Row {
+    const T* x;
+    int head, nv, tail, V;
+    __device__ __forceinline__ Row(const LogprobArgs& a, int64_t r) {
+        x = static_cast<const T*>(a.x) + r * a.stride;
+        V = a.vocab;
+        head = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
+        if (head > V) head = V;
+        nv = (V - head) / Vec<T>::n;
+        tail = head + nv * Vec<T>::n;
+    }
+    __device__ __forceinline__ int first(int i) const { return head + i * Vec<T>::n; }
+    __device__ __forceinline__ uint4 vec(int i) const {
+        return __ldg(reinterpret_cast<const uint4*>(x + head) + i);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void widen(uint4 w, float2 (&f)[Vec<T>::n / 2]) {
+    float g[Vec<T>::n];
+    constexpr int k = 4 / (int)sizeof(T);
+    unpack32(w.x, g, T{});
+    unpack32(w.y, g + k, T{});
+    unpack32(w.z, g + 2 * k, T{});
+    unpack32(w.w, g + 3 * k, T{});
+#pragma unroll
+    for (int i = 0; i < Vec<T>::n / 2; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
+}
+
+// Largest of the elements of N words: 16-bit pairs compared as they are.
+// NaN is passed over, as by fmaxf.
+template <int N>
+__device__ __forceinline__ float max_of(const uint4 (&w)[N], float) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(w[i].x), __uint_as_float(w[i].y)),
+                           fmaxf(__uint_as_float(w[i].z), __uint_as_float(w[i].w))));
+    return m;
+}
+template <int N, typename T, typename T2>
+__device__ __forceinline__ float max_of_pairs(const uint4 (&w)[N]) {
+    auto p = [](const uint32_t& v) { return *reinterpret_cast<const T2*>(&v); };
+    T2 m = __hmax2(__hmax2(p(w[0].x), p(w[0].y)), __hmax2(p(w[0].z), p(w[0].w)));
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+        m = __hmax2(m, __hmax2(__hmax2(p(w[i].x), p(w[i].y)), __hmax2(p(w[i].z), p(w[i].w))));
+    return fmaxf(fmaxf(to_f(m.x), to_f(m.y)), -INFINITY);  // all NaN: -inf
+}
+template <int N>
+__device__ __forceinline__ float max_of(const uint4 (&w)[N], __nv_bfloat16) {
+    return max_of_pairs<N, __nv_bfloat16, __nv_bfloat162>(w);
+}
+template <int N>
+__device__ __forceinline__ float max_of(const uint4 (&w)[N], __half) {
+    return max_of_pairs<N, __half, __half2>(w);
+}
+// A vector of -inf, which adds nothing.
+template <typename T>
+__device__ __forceinline__ uint4 nothing() {
+    constexpr float kInf[2] = {-INFINITY, -INFINITY};
+    const uint32_t v = pack32(kInf, T{});
+    return make_uint4(v, v, v, v);
+}
+
+// The threads of one row: a warp, or the CTA.
+template <int NT>
+struct Team {
+    static constexpr int kWarps = NT / 32;
+    // Vectors that a thread sums at a time, and as many again on their way: two
+    // where a team has little for each thread and latency counts.
+    static constexpr int kUnroll = NT >= 256 ? 2 : 4;
+    static constexpr int kCap = NT == 32 ? 128 : 512;   // candidates
+    static constexpr int kSegs = 16;                    // segments of a thread's elements
+    struct Shared {
+        float seg[kSegs * NT];
+        unsigned long long list[kCap];
+        float group[32];
+        float s[kWarps], t[kWarps];
+        unsigned long long key[kWarps];
+        int count;
+    };
+    static __device__ __forceinline__ void sync() {
+        if constexpr (NT == 32) __syncwarp();
+        else __syncthreads();
+    }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// The lanes' values in falling order over the lanes (bitonic).
+__device__ __forceinline__ float sort_falling(float v, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int o = k >> 1; o > 0; o >>= 1) {
+            const float w = __shfl_xor_sync(0xffffffffu, v, o);
+            const bool larger = ((lane & o) == 0) == ((lane & k) == 0);
+            v = larger ? fmaxf(v, w) : fminf(v, w);
+        }
+    return v;
+}
+
+// The top_k largest one after the other: each thread's largest, the team's
+// largest, and its owner looks for its next one below it.
+template <typename T, int NT>
+__device__ __noinline__ void top_by_rounds(Row<T> row, int top_k, int32_t* ids, int tid,
+                                           typename Team<NT>::Shared& sh) {
+    constexpr int EV = Vec<T>::n;
+    unsigned long long below = ~0ull, best = 0;
+    for (int k = 0; k < top_k; ++k) {
+        if (k == 0 || best == below) {
+            best = 0;
+            auto look = [&](int j) {
+                const unsigned long long c = key_of(to_f(row.x[j]), j);
+                if (k == 0 || c < below) best = max_key(best, c);
+            };
+            if (tid < row.head) look(tid);
+            for (int i = tid; i < row.nv; i += NT)
+                for (int e = 0; e < EV; ++e) look(row.first(i) + e);
+            if (tid < row.V - row.tail) look(row.tail + tid);
+        }
+        unsigned long long b = best;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) b = max_key(b, __shfl_xor_sync(0xffffffffu, b, o));
+        if constexpr (NT > 32) {
+            if ((tid & 31) == 0) sh.key[tid >> 5] = b;
+            __syncthreads();
+            for (int w = 0; w < NT / 32; ++w) b = max_key(b, sh.key[w]);
+            __syncthreads();
+        }
+        below = b;
+        if (tid == 0) ids[k] = (int)~(uint32_t)b;
+    }
+}
+
+// S and T with d = x - m, in base 2 units, for the rows whose x log2 e may overflow.
+template <typename T, int NT>
+__device__ __noinline__ void sums_from_differences(Row<T> row, int tid, float m,
+                                                   typename Team<NT>::Shared& sh, float* s_out, float* t_out) {
+    float s = 0.0f, t = 0.0f;
+    for (int j = tid; j < row.V; j += NT) {
+        const float d = (to_f(row.x[j]) - m) * kLog2e, e = ex2_approx(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, kLeast), t);
+    }
+    s = warp_sum(s);
+    t = warp_sum(t);
+    if constexpr (NT > 32) {
+        __syncthreads();  // the first sums have been read
+        if ((tid & 31) == 0) {
+            sh.s[tid >> 5] = s;
+            sh.t[tid >> 5] = t;
+        }
+        __syncthreads();
+        s = t = 0.0f;
+        for (int w = 0; w < NT / 32; ++w) {
+            s += sh.s[w];
+            t += sh.t[w];
+        }
+    }
+    *s_out = s;
+    *t_out = t;
+}
+
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256 ? 5 : 1) k_token_logprobs(LogprobArgs a) {
+    using Tm = Team<NT>;
+    constexpr int EV = Vec<T>::n;
+    constexpr int kTeams = NT < 128 ? 128 / NT : 1;  // rows at a time
+    __shared__ typename Tm::Shared shared[kTeams];
+    const int tid = threadIdx.x % NT, lane = tid & 31, warp = tid >> 5;
+    typename Tm::Shared& sh = shared[threadIdx.x / NT];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t stride = (int64_t)gridDim.x * kTeams;
+    const int64_t r0 = (int64_t)blockIdx.x * kTeams + threadIdx.x / NT;
+    constexpr int kUnroll = Tm::kUnroll;
+    constexpr int kBatch = NT * kUnroll;  // vectors that the team takes at a time
+    // A row's b-th batch; behind the row: nothing.
+    auto fetch = [&](const Row<T>& row, int b, uint4 (&w)[kUnroll]) {
+        const uint4* p = reinterpret_cast<const uint4*>(row.x + row.head) + b * kBatch + tid;
+        if ((b + 1) * kBatch <= row.nv) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) w[u] = __ldg(p + u * NT);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                w[u] = nothing<T>();
+                if (b * kBatch + u * NT + tid < row.nv) w[u] = __ldg(p + u * NT);
+            }
+        }
+    };
+    // The next batch is on its way while one is summed, the next row's first
+    // batch and token while a row is finished: a row's sums, joins and
+    // alternatives are a chain of latencies that would otherwise follow its loads.
+    uint4 ahead[kUnroll];
+    int tok_ahead = -1;
+    if (r0 < a.n_rows) {
+        if (tid == 0 && a.logprob) tok_ahead = __ldg(a.tokens + r0);
+        fetch(Row<T>(a, r0), 0, ahead);
+    }
+    for (int64_t r = r0; r < a.n_rows; r += stride) {
+        const Row<T> row(a, r);
+        Stat st = {reference_of(-INFINITY), {0.0f, 0.0f}, {0.0f, 0.0f}};
+        float top = -INFINITY;  // the thread's largest
+        // The ends: at most one scalar of each per thread.  The given token's logit.
+        T end_head = from_f<T>(-INFINITY), end_tail = end_head, x_tok = from_f<T>(NAN);
+        if (tid < row.head) end_head = row.x[tid];
+        if (tid < row.V - row.tail) end_tail = row.x[row.tail + tid];
+        const int tok = tok_ahead;
+        if (tok >= 0 && tok < row.V) x_tok = row.x[tok];
+
+        const int batches = row.nv > kBatch ? (row.nv + kBatch - 1) / kBatch : 1;
+        const int per = (batches + Tm::kSegs - 1) / Tm::kSegs;  // batches of a segment
+        int n_segs = 0;
+        float seg = -INFINITY;
+        for (int b = 0, in_seg = 0; b < batches; ++b) {
+            uint4 w[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) w[u] = ahead[u];
+            if (b + 1 < batches) {
+                fetch(row, b + 1, ahead);
+            } else if (r + stride < a.n_rows) {
+                if (tid == 0 && a.logprob) tok_ahead = __ldg(a.tokens + r + stride);
+                fetch(Row<T>(a, r + stride), 0, ahead);
+            }
+            const float m = max_of(w, T{});
+            if ((b + 1) * kBatch <= row.nv) {
+                float2 f[kUnroll * EV / 2];
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+                    widen<T>(w[u], *reinterpret_cast<float2(*)[EV / 2]>(f + u * EV / 2));
+                add<kUnroll * EV>(st, f, m);
+            } else {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+                    if (b * kBatch + u * NT < row.nv) {
+                        float2 f[EV / 2];
+                        widen<T>(w[u], f);
+                        add<EV>(st, f, m);
+                    }
+            }
+            if (TOP) {
+                seg = fmaxf(seg, m);
+                if (++in_seg == per || b + 1 == batches) {
+                    sh.seg[n_segs++ * NT + tid] = seg;
+                    seg = -INFINITY;
+                    in_seg = 0;
+                }
+            }
+            top = fmaxf(top, m);
+        }
+        float2 ends[1] = {{to_f(end_head), to_f(end_tail)}};
+        if (tid < row.head || tid < row.V - row.tail) {
+            const float m = fmaxf(ends[0].x, ends[0].y);
+            add<2>(st, ends, m);
+            top = fmaxf(top, m);
+        }
+
+        // Maximum of the row, then the sums relative to its reference.
+        float m = warp_max(top);
+        if constexpr (NT > 32) {
+            float g = top;
+#pragma unroll
+            for (int o = 1; o < NT / 32; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+            if (tid % (NT / 32) == 0) sh.group[tid / (NT / 32)] = g;
+            if (TOP && tid == 0) sh.count = 0;
+            __syncthreads();
+            m = warp_max(sh.group[lane]);
+        }
+        float ref = reference_of(m);
+        st.raise(ref);
+        float s = warp_sum(st.s.x + st.s.y), t = warp_sum(st.t.x + st.t.y);
+        if constexpr (NT > 32) {
+            if (lane == 0) {
+                sh.s[warp] = s;
+                sh.t[warp] = t;
+            }
+            __syncthreads();
+            s = t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < Tm::kWarps; ++w) {
+                s += sh.s[w];
+                t += sh.t[w];
+            }
+        } else if (TOP) {
+            if (lane == 0) sh.count = 0;
+            __syncwarp();
+        }
+        bool bad = false, huge = false;
+        if (!(fabsf(m) <= kHuge && s <= 3e38f)) {  // rare: no distribution, or logits near the type's limits
+            huge = true;
+            sums_from_differences<T, NT>(row, tid, m, sh, &s, &t);
+            bad = fabsf(m) == INFINITY || s != s;
+        }
+        const float log_s = log2f(s);
+        // ln sum e^(x - m): the sums refer to ref, which m log2 e is below by the FMA's value.
+        const float ln_s = (log_s - (huge ? 0.0f : fmaf(m, kLog2e, -ref))) * kLn2;
+        auto log_prob = [&](float x) { return bad ? (float)NAN : (x - m) - ln_s; };
+        if (tid == 0) {
+            if (a.entropy) a.entropy[r] = bad ? NAN : (log_s - t / s) * kLn2;
+            if (a.logprob) {
+                if (tok < -1 || tok >= row.V) atomicOr(a.err, CBX_EFLAG_TOKEN_OOB);
+                a.logprob[r] = log_prob(to_f(x_tok));  // NaN without a token
+            }
+        }
+        if constexpr (TOP) {
+            float tau = m;
+            if (a.top_k > 1)
+                tau = __shfl_sync(0xffffffffu, sort_falling(NT > 32 ? sh.group[lane] : top, lane), a.top_k - 1);
+            // Puts the elements of the mask, first + bit, on the list.
+            auto offer = [&](uint32_t mask, int first) {
+                if (!mask) return;
+                int at = atomicAdd(&sh.count, __popc(mask));
+                for (; mask; mask &= mask - 1, ++at) {
+                    const int j = first + __ffs(mask) - 1;
+                    if (at < Tm::kCap) sh.list[at] = key_of(to_f(row.x[j]), j);
+                }
+            };
+            if (!bad && top >= tau && (tau != -INFINITY || row.V <= Tm::kCap)) {
+                if (tid < row.head) offer(ends[0].x >= tau, tid);
+                if (tid < row.V - row.tail) offer(ends[0].y >= tau, row.tail + tid);
+                uint32_t todo = 0;
+                for (int q = 0; q < n_segs; ++q) todo |= (sh.seg[q * NT + tid] >= tau ? 1u : 0u) << q;
+                while (todo) {
+                    int i = (__ffs(todo) - 1) * per * kUnroll;
+                    todo &= todo - 1;
+                    for (const int i1 = i + per * kUnroll; i < i1; ++i) {
+                        const int v = tid + i * NT;
+                        if (v >= row.nv) break;
+                        const uint4 w[1] = {row.vec(v)};
+                        if (max_of(w, T{}) < tau) continue;
+                        float2 f[EV / 2];
+                        widen<T>(w[0], f);
+                        uint32_t mask = 0;
+#pragma unroll
+                        for (int e = 0; e < EV / 2; ++e)
+                            mask |= (f[e].x >= tau ? 1u : 0u) << (2 * e) | (f[e].y >= tau ? 2u : 0u) << (2 * e);
+                        offer(mask, row.first(v));
+                    }
+                }
+            }
+            Tm::sync();
+            const int n = sh.count;
+            if (n >= a.top_k && n <= Tm::kCap) {
+                for (int i = tid; i < n; i += NT) {
+                    const unsigned long long key = sh.list[i];
+                    int rank = 0;
+                    for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
+                    if (rank < a.top_k) {
+                        a.top_ids[r * a.top_k + rank] = (int)~(uint32_t)key;
+                        a.top_logprobs[r * a.top_k + rank] = log_prob(value_of(key));
+                    }
+                }
+            } else {
+                int32_t* ids = a.top_ids + r * a.top_k;
+                top_by_rounds<T, NT>(row, a.top_k, ids, tid, sh);
+                if (tid == 0)
+                    for (int k = 0; k < a.top_k; ++k)
+                        a.top_logprobs[r * a.top_k + k] = log_prob(to_f(row.x[ids[k]]));
+            }
+        }
+        Tm::sync();  // the next row uses the shared arrays again
+    }
+}
+
+template <typename T, int NT>
+int run_team(const LogprobArgs& a, cudaStream_t st) {
+    constexpr int kCta = NT < 128 ? 128 : NT;
+    auto kern = a.top_k > 0 ? k_token_logprobs<T, NT, true> : k_token_logprobs<T, NT, false>;
+    // The fewest CTAs that give each the same number of rows within one: no last
+    // round of rows on a part of the resident warps.
+    const int64_t ctas = (a.n_rows + kCta / NT - 1) / (kCta / NT);
+    const int64_t most = (int64_t)num_sms() * occupancy(kern, kCta);
+    const int64_t rounds = (ctas + most - 1) / most;
+    const unsigned grid = (unsigned)((ctas + rounds - 1) / rounds);
+    return launch_status(launch(kern, dim3(grid), dim3(kCta), 0, st, a),
+                         "cbx_token_logprobs");
+}
+
+// Threads of a row.  A warp costs least per row, but needs many rows to fill
+// the GPU and is slow on a long one; a whole CTA is quickest on a single row.
+// Measured in us (B200; 32 / 128 / 256 / 512 threads a row):
+//   1 x 6563 f32          7.6 / 5.2 / 4.5 / 4.5
+//   1 x 50276 f32        38.7 / 12.0 / 9.9 / 7.2
+//   256 x 6563 f32       10.6 / 6.9 / 6.2 / 8.6
+//   1100 x 6563 f16      12.0 / 14.9 / 14.7 / 27.4
+//   1100 x 50276 f16     64.2 / 45.1 / 39.6 / 60.0
+//   2048 x 50276 f16    110.2 / 53.6 / 62.7 / 111.8
+//   4200 x 20000 bf16    66.8 / 57.5 / 61.6 / 131.4
+//   8192 x 6563 bf16     29.0 / 46.1 / 65.4 / 160.9
+// The warp's list holds the candidates of up to 24 alternatives (about 32 ln(1 /
+// (1 - k / 32)) of them, 44 for 24).
 template <typename T>
 int run_logprobs(const LogprobArgs& a, cudaStream_t st) {
-    const int64_t most = (int64_t)num_sms() * occupancy(k_token_logprobs<T>, kThreads);
-    const unsigned grid = (unsigned)(a.n_rows < most ? a.n_rows : most);
-    return launch_status(launch(k_token_logprobs<T>, dim3(grid), dim3(kThreads), 0, st, a),
-                         "cbx_token_logprobs");
+    const int64_t rows = a.n_rows, sms = num_sms();
+    const bool is_short = a.vocab <= 2048 * Vec<T>::n;  // up to 32 KB
+    if (rows <= sms) return run_team<T, 512>(a, st);
+    if (rows >= 7 * sms && is_short && a.top_k <= 24) return run_team<T, 32>(a, st);
+    if (rows >= 10 * sms) return run_team<T, 128>(a, st);
+    return run_team<T, 256>(a, st);
 }
 
 }  // namespace

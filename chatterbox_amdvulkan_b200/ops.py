@@ -618,17 +618,35 @@ def _paged_cache(cache_k: torch.Tensor, cache_v: torch.Tensor):
     return P, S, Hk, hd, page_stride
 
 
-def _here(t: torch.Tensor, name: str, dtype=None) -> int:
-    """Address of a CUDA tensor of any strides (the caller checks them)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor (libcbx_ops has no CPU path)")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the call runs on "
-                         f"cuda:{torch.cuda.current_device()}: all tensors of a call must "
-                         "share its device")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+# A decode step calls these wrappers once per layer, so they check their tensors in few Python
+# operations (a call of the smallest sizes is bound by them, not by its kernel): the device index,
+# type and contiguity here, and the full message only where one of them is wrong.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _addr(t: torch.Tensor | None, dev: int, name: str, dtype=None, dense: bool = True):
+    """Address of a tensor of a call on CUDA device `dev` (None stays None); `dense` False: the
+    caller has checked the strides."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or dev < 0 or \
+            (dtype is not None and t.dtype is not dtype) or (dense and not t.is_contiguous()):
+        _dev(t, name, dtype)                       # raises what is wrong
+        raise ValueError(f"{name} must be a CUDA tensor of the call's device")
     return t.data_ptr()
+
+
+def _call(fn: str, *args) -> None:
+    """_lib.call with the function looked up once."""
+    f = _FNS.get(fn)
+    if f is None:
+        f = _FNS[fn] = getattr(_lib.load(), fn)
+    status = f(*args)
+    if status != 0:
+        _lib.check(fn, status)
+
+
+_FNS: dict = {}
 
 
 def _err_word(err: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
@@ -687,15 +705,16 @@ def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torc
         rows = [new(max_rows) for _ in range(4)] + [new(n_reqs + 1)]
         state = (block_table, n_blocks, free_list, n_free)
         out = (*rows, *(state if in_place else map(torch.empty_like, state)))
+    i32, dev = torch.int32, seq_lens.get_device()
+    lens_p = _addr(seq_lens, dev, "seq_lens", i32)
     err = _err_word(err, seq_lens)
-    i32 = torch.int32
-    slots, positions, row_reqs, row_lens, row_start, table_o, blocks_o, free_o, n_free_o = (
-        _dev(t, "out", i32) for t in out)
-    _lib.call("cbx_paged_plan", _dev(seq_lens, "seq_lens", i32), _dev(n_new, "n_new", i32), n_reqs,
-              max_blocks, int(page_size), free_list.numel(), _dev(block_table, "block_table", i32),
-              _dev(n_blocks, "n_blocks", i32), _dev(free_list, "free_list", i32),
-              _dev(n_free, "n_free", i32), table_o, blocks_o, free_o, n_free_o, max_rows, slots,
-              positions, row_reqs, row_lens, row_start, _dev(err, "err", i32), _stream(seq_lens))
+    slots, positions, row_reqs, row_lens, row_start, table_o, blocks_o, free_o, n_free_o = [
+        _addr(t, dev, "out", i32) for t in out]
+    _call("cbx_paged_plan", lens_p, _addr(n_new, dev, "n_new", i32), n_reqs, max_blocks,
+          int(page_size), free_list.numel(), _addr(block_table, dev, "block_table", i32),
+          _addr(n_blocks, dev, "n_blocks", i32), _addr(free_list, dev, "free_list", i32),
+          _addr(n_free, dev, "n_free", i32), table_o, blocks_o, free_o, n_free_o, max_rows, slots,
+          positions, row_reqs, row_lens, row_start, _addr(err, dev, "err", i32), _raw_stream(dev))
     return PagedPlan(*out, err)
 
 
@@ -728,14 +747,16 @@ def qkv_kv_append_paged(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: t
         raise ValueError(f"bias has {bias.numel()} entries, expected {width}")
     if q_out is not None and (q_out.numel() != n_rows * q_dim or q_out.dtype != qkv.dtype):
         raise ValueError(f"q_out must hold {n_rows} x {q_dim} values of {qkv.dtype}")
+    dev = qkv.get_device()
+    qkv_p = _addr(qkv, dev, "qkv", dense=False)
     if q_out is None and with_q:
-        q_out = torch.empty((n_rows, q_dim), dtype=qkv.dtype, device=qkv.device)
+        q_out = qkv.new_empty((n_rows, q_dim))
     err = _err_word(err, qkv)
-    _lib.call("cbx_qkv_kv_append_paged", _here(qkv, "qkv"), _cbx_type(qkv), stride,
-              _dev(bias, "bias", torch.float32), n_rows, q_dim, kv_dim,
-              _dev(slots, "slots", torch.int32), _here(cache_k, "cache_k"),
-              _here(cache_v, "cache_v"), _cbx_type(cache_k), P, S, page_stride,
-              _dev(q_out, "q_out"), _dev(err, "err", torch.int32), _stream(qkv))
+    _call("cbx_qkv_kv_append_paged", qkv_p, _cbx_type(qkv), stride,
+          _addr(bias, dev, "bias", torch.float32), n_rows, q_dim, kv_dim,
+          _addr(slots, dev, "slots", torch.int32), _addr(cache_k, dev, "cache_k", dense=False),
+          _addr(cache_v, dev, "cache_v", dense=False), _cbx_type(cache_k), P, S, page_stride,
+          _addr(q_out, dev, "q_out"), _addr(err, dev, "err", torch.int32), _raw_stream(dev))
     return q_out, err
 
 
@@ -771,29 +792,34 @@ def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torc
         raise ValueError(f"seq_lens and row_reqs must hold one entry for each of {n_rows} rows")
     if row_reqs is None and n_reqs < n_rows:
         raise ValueError(f"block_table has {n_reqs} rows for {n_rows} rows of q")
-    if out is None:
-        out = torch.empty((n_rows, H, hd), dtype=q.dtype, device=q.device)
-    elif out.numel() != n_rows * H * hd or out.dtype != q.dtype:
+    if out is not None and (out.numel() != n_rows * H * hd or out.dtype is not q.dtype):
         raise ValueError(f"out must hold {n_rows} x {H} x {hd} values of {q.dtype}")
+    dev = q.get_device()
+    q_p = _addr(q, dev, "q", dense=False)
+    if out is None:
+        out = q.new_empty((n_rows, H, hd))
     lse = torch.empty((n_rows, H), dtype=torch.float32, device=q.device) if return_lse else None
     ct = _cbx_type(cache_k)
-    q_ptr = _here(q, "q")
-    need = _workspace_bytes(n_rows, H, Hk, hd, max_blocks, S, ct)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    need = _workspace_bytes(dev, n_rows, H, Hk, hd, max_blocks, S, ct)
+    ws_p, ws_bytes = None, 0
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws_p, ws_bytes = _addr(workspace, dev, "workspace"), workspace.nbytes
     err = _err_word(err, q)
-    _lib.call("cbx_paged_decode_attention", q_ptr, _cbx_type(q), q_stride,
-              _here(cache_k, "cache_k"), _here(cache_v, "cache_v"), ct, P, S, page_stride,
-              _dev(block_table, "block_table", torch.int32), n_reqs, max_blocks,
-              _dev(row_reqs, "row_reqs", torch.int32), _dev(seq_lens, "seq_lens", torch.int32),
-              n_rows, H, Hk, hd, float(hd ** -0.5 if scale is None else scale), _dev(out, "out"),
-              _dev(lse, "lse"), _dev(workspace, "workspace") if need else None,
-              workspace.numel() * workspace.element_size() if need else 0,
-              _dev(err, "err", torch.int32), _stream(q))
+    i32 = torch.int32
+    _call("cbx_paged_decode_attention", q_p, _cbx_type(q), q_stride,
+          _addr(cache_k, dev, "cache_k", dense=False), _addr(cache_v, dev, "cache_v", dense=False),
+          ct, P, S, page_stride, _addr(block_table, dev, "block_table", i32), n_reqs, max_blocks,
+          _addr(row_reqs, dev, "row_reqs", i32), _addr(seq_lens, dev, "seq_lens", i32), n_rows, H,
+          Hk, hd, hd ** -0.5 if scale is None else scale, _addr(out, dev, "out"),
+          _addr(lse, dev, "lse"), ws_p, ws_bytes, _addr(err, dev, "err", i32), _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
-def _workspace_bytes(n_rows, n_heads, n_kv_heads, head_dim, max_blocks, page_size, cache_type):
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(dev, n_rows, n_heads, n_kv_heads, head_dim, max_blocks, page_size, cache_type):
+    """Per device: the split depends on its number of SMs."""
     n = _lib.load().cbx_paged_decode_attention_workspace(n_rows, n_heads, n_kv_heads, head_dim,
                                                          max_blocks, page_size, cache_type)
     if n < 0:
@@ -805,8 +831,9 @@ def paged_decode_attention_workspace(n_rows: int, n_heads: int, n_kv_heads: int,
                                      max_blocks: int, page_size: int,
                                      cache_dtype: torch.dtype = torch.float32) -> int:
     """Bytes of workspace ``paged_decode_attention`` needs for these sizes on the current device."""
-    return _workspace_bytes(int(n_rows), int(n_heads), int(n_kv_heads), int(head_dim),
-                            int(max_blocks), int(page_size), _TORCH_TO_CBX[cache_dtype])
+    return _workspace_bytes(torch.cuda.current_device(), int(n_rows), int(n_heads),
+                            int(n_kv_heads), int(head_dim), int(max_blocks), int(page_size),
+                            _TORCH_TO_CBX[cache_dtype])
 
 
 # ------------------------------------------------- token log probabilities --
@@ -839,14 +866,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top_k: int
         raise ValueError(f"logits' rows overlap: stride {stride} < {vocab}")
     if tokens is not None and tokens.numel() != n_rows:
         raise ValueError(f"tokens has {tokens.numel()} entries for {n_rows} rows")
-    dev = logits.device
-    lp = torch.empty(n_rows, dtype=torch.float32, device=dev) if tokens is not None else None
-    entropy = torch.empty(n_rows, dtype=torch.float32, device=dev)
-    ids = torch.empty((n_rows, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((n_rows, top_k), dtype=torch.float32, device=dev)
+    dev = logits.get_device()
+    x_p = _addr(logits, dev, "logits", dense=False)
+    f32, i32, device = torch.float32, torch.int32, logits.device
+    lp = torch.empty(n_rows, dtype=f32, device=device) if tokens is not None else None
+    entropy = torch.empty(n_rows, dtype=f32, device=device)
+    ids = torch.empty((n_rows, top_k), dtype=i32, device=device)
+    top = torch.empty((n_rows, top_k), dtype=f32, device=device)
     err = _err_word(err, logits)
-    _lib.call("cbx_token_logprobs", _here(logits, "logits"), _cbx_type(logits), stride, n_rows,
-              vocab, _dev(tokens, "tokens", torch.int32), top_k, _dev(lp, "logprobs"),
-              _dev(entropy, "entropy"), _dev(ids, "top_ids"), _dev(top, "top_logprobs"),
-              _dev(err, "err", torch.int32), _stream(logits))
+    _call("cbx_token_logprobs", x_p, _cbx_type(logits), stride, n_rows, vocab,
+          _addr(tokens, dev, "tokens", i32), top_k, _addr(lp, dev, "logprobs"), entropy.data_ptr(),
+          ids.data_ptr(), top.data_ptr(), _addr(err, dev, "err", i32), _raw_stream(dev))
     return TokenLogprobs(lp, entropy, ids, top, err)
