@@ -11,18 +11,26 @@
 // end.  Exponentials are base 2 (scale log2 e is folded into q).
 //
 // Bound by HBM: each key and value is read once and takes 2 FMAs per query
-// head.  A key row of one kv head is VL 16-byte vectors, one per lane, so a
-// warp reads 32 / VL keys per load instruction and holds U loads of keys and
-// U of values in flight: no shared memory between HBM and the FMAs.
+// head.  Two kernels, both with whole tiles of keys and values in flight per
+// warp and no CTA barrier in the loop:
+//  - k_attend_fma: one or two query heads per kv head, or an f32 cache.  A key
+//    row of one kv head is VL 16-byte vectors, one per lane, so a warp reads
+//    32 / VL keys per load instruction.  f32 FMAs.
+//  - k_attend_mma: 16-bit caches and more query heads per kv head, where the
+//    FMAs and the conversions to f32 would bound it.  mma.sync of 16 rows: the
+//    up to 8 query heads of a kv head, twice.
+//
+// The keys of a row are split over the CTAs of a cluster (up to 8), which join
+// their states through distributed shared memory, or, where even that leaves
+// SMs idle, over more CTAs with partial states in the workspace and a second
+// launch that joins them.
 #include "cbx_common.cuh"
 
 namespace cbx {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxSplits = 64;
-constexpr int kMinKeys = 256;  // keys of a split at the least
 
 struct AttnArgs {
     const void* q;
@@ -30,7 +38,7 @@ struct AttnArgs {
     int64_t q_stride;
     const void* ck;
     const void* cv;
-    int n_pages, page_size;
+    int n_pages, page_size, page_shift;  // page_shift: log2(page_size), -1 where it is none
     int page_rows;  // page_stride in rows of kv_dim
     int64_t kv_dim;
     const int32_t* table;
@@ -38,12 +46,13 @@ struct AttnArgs {
     const int32_t* row_reqs;
     const int32_t* seq_lens;
     int n_heads, n_kv, group, head_dim;
-    int chunks;  // chunks of G query heads per kv head
+    int chunks;  // chunks of query heads per kv head
     float scale_log2;
     void* out;
     float* lse;
-    float* part;  // [rows][heads][splits][2 + head_dim rounded up to 4]: m, l, -, -, acc
+    float* part;  // [rows][heads][splits][state]
     int splits;
+    bool cluster;  // the splits are a cluster
     int32_t* err;
 };
 
@@ -64,48 +73,157 @@ __device__ __forceinline__ float rescale(float a, float b) {
     return a == -INFINITY ? 0.0f : ex2_approx(a - b);
 }
 
+// Natural logarithm of the sum that (m, l) stand for; -inf without keys.
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l != 0.0f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+// Shared memory of the cluster's CTA `rank` at this CTA's address `p`.
+__device__ __forceinline__ uint32_t peer_smem(uint32_t p, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_peer(uint32_t p) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(p));
+    return v;
+}
+
 // One state (m, l, acc) of a row and head.
 constexpr int kStateHead = 4;  // floats before acc: m, l, two unused
 __host__ __device__ inline int state_floats(int head_dim) { return kStateHead + head_dim; }
 
+// What a CTA works on: a row, one kv head with up to G of its query heads, and
+// one split's keys [lo, hi), whole steps of the CTA.
+struct Work {
+    int row, kvh, head0, heads, lo, hi;
+    const int32_t* table;
+    int flags;
+    __device__ __forceinline__ Work(const AttnArgs& a, int chunk_heads, int step) {
+        row = blockIdx.z;
+        kvh = blockIdx.y / a.chunks;
+        const int first = blockIdx.y % a.chunks * chunk_heads;
+        head0 = kvh * a.group + first;
+        heads = a.group - first < chunk_heads ? a.group - first : chunk_heads;
+        flags = 0;
+        int req = a.row_reqs ? a.row_reqs[row] : row;
+        int len = a.seq_lens[row];
+        const int64_t cap = (int64_t)a.max_blocks * a.page_size;
+        if (len < 0 || len > cap) {
+            flags |= CBX_EFLAG_LENGTH;
+            len = len < 0 ? 0 : (int)cap;
+        }
+        if (req < 0 || req >= a.n_reqs) {
+            flags |= CBX_EFLAG_PAGE_OOB;
+            req = 0;
+            len = 0;
+        }
+        table = a.table + (int64_t)req * a.max_blocks;
+        const int64_t steps = ((int64_t)len + step - 1) / step;
+        const int64_t from = steps * blockIdx.x / a.splits * step;
+        const int64_t to = steps * (blockIdx.x + 1) / a.splits * step;
+        lo = from < len ? (int)from : len;
+        hi = to < len ? (int)to : len;
+    }
+    // Cache row of a key; -1 behind the split's last and on a bad page.
+    __device__ __forceinline__ int find(const AttnArgs& a, int64_t key) {
+        if (key >= hi) return -1;
+        const int blk = a.page_shift >= 0 ? (int)key >> a.page_shift : (int)key / a.page_size;
+        const int page = __ldg(table + blk);
+        if (page < 0 || page >= a.n_pages) {
+            flags |= CBX_EFLAG_PAGE_OOB;
+            return -1;
+        }
+        return page * a.page_rows + ((int)key - blk * a.page_size);
+    }
+};
+
+// Joins the states [W][G][state] of the CTA's warps (in shared memory, written
+// by all of them) and the CTAs of the row, and stores the result.
+template <int W, int G>
+__device__ __forceinline__ void finish(const AttnArgs& a, const Work& w, float* states) {
+    const int hd = a.head_dim, sf = state_floats(hd);
+    float* own = states + W * G * sf;  // [G][state] of this CTA
+    __syncthreads();
+    for (int i = threadIdx.x; i < w.heads * hd; i += W * 32) {
+        const int g = i / hd, e = i % hd;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < W; ++k) mm = fmaxf(mm, states[(k * G + g) * sf]);
+        float ll = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float* st = states + (k * G + g) * sf;
+            const float c = rescale(st[0], mm);
+            ll += c * st[1];
+            o += c * st[kStateHead + e];
+        }
+        const int64_t rh = (int64_t)w.row * a.n_heads + w.head0 + g;
+        if (a.splits > 1) {
+            float* st = a.cluster ? own + g * sf : a.part + (rh * a.splits + blockIdx.x) * sf;
+            if (e == 0) {
+                st[0] = mm;
+                st[1] = ll;
+            }
+            st[kStateHead + e] = o;
+        } else {
+            store_elem(a.out, a.q_type, rh * hd + e, ll != 0.0f ? o / ll : 0.0f);
+            if (a.lse && e == 0) a.lse[rh] = lse_of(mm, ll);
+        }
+    }
+    if (!a.cluster) return;
+    cluster_sync();
+    // Each CTA of the cluster joins its share of the values.
+    for (int i = blockIdx.x * (W * 32) + threadIdx.x; i < w.heads * hd; i += a.splits * (W * 32)) {
+        const int g = i / hd, e = i % hd;
+        const uint32_t st = smem_addr(own + g * sf);
+        float m[kMaxCluster], l[kMaxCluster], v[kMaxCluster];
+        float mm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            if (k < a.splits) {
+                const uint32_t peer = peer_smem(st, k);
+                m[k] = ld_peer(peer);
+                l[k] = ld_peer(peer + 4);
+                v[k] = ld_peer(peer + 4 * (kStateHead + e));
+                mm = fmaxf(mm, m[k]);
+            }
+        }
+        float ll = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            if (k < a.splits) {
+                const float c = rescale(m[k], mm);
+                ll += c * l[k];
+                o += c * v[k];
+            }
+        }
+        const int64_t rh = (int64_t)w.row * a.n_heads + w.head0 + g;
+        store_elem(a.out, a.q_type, rh * hd + e, ll != 0.0f ? o / ll : 0.0f);
+        if (a.lse && e == 0) a.lse[rh] = lse_of(mm, ll);
+    }
+    cluster_sync();  // no CTA leaves while another reads its states
+}
+
+constexpr int kFmaWarps = 8;
+
 template <typename TC, int VL, int VPL, int G>
-__global__ void __launch_bounds__(kThreads) k_paged_attention(AttnArgs a) {
+__global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
     constexpr int EV = Vec<TC>::n;        // elements per 16-byte vector
     constexpr int EL = EV * VPL;          // elements of the head per lane
     constexpr int U = VL < 8 ? VL : 8;    // loads in flight
     constexpr int KPL = 32 / VL;          // keys per load
     constexpr int TILE = KPL * U;         // keys per warp and step
-    extern __shared__ float smem[];       // [kWarps][G][state]
-    const int split = blockIdx.x, hc = blockIdx.y, row = blockIdx.z;
-    const int kvh = hc / a.chunks, chunk = hc % a.chunks;
+    constexpr int step = TILE * kFmaWarps;
+    extern __shared__ float smem[];       // states
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vl = lane % VL, kg = lane / VL;
     const int hd = a.head_dim;
-    const int head0 = kvh * a.group + chunk * G;
-    const int heads = a.group - chunk * G < G ? a.group - chunk * G : G;
     grid_dep_wait();
     grid_dep_launch();
-
-    int flags = 0;
-    int req = a.row_reqs ? a.row_reqs[row] : row;
-    int len = a.seq_lens[row];
-    const int64_t cap = (int64_t)a.max_blocks * a.page_size;
-    if (len < 0 || len > cap) {
-        flags |= CBX_EFLAG_LENGTH;
-        len = len < 0 ? 0 : (int)cap;
-    }
-    if (req < 0 || req >= a.n_reqs) {
-        flags |= CBX_EFLAG_PAGE_OOB;
-        req = 0;
-        len = 0;
-    }
-    const int32_t* table = a.table + (int64_t)req * a.max_blocks;
-    // This split's keys: whole tiles of the CTA, evenly over the splits.
-    const int64_t step = (int64_t)TILE * kWarps;
-    const int64_t tiles = (len + step - 1) / step;
-    const int64_t lo = tiles * split / a.splits * step;
-    int64_t hi64 = tiles * (split + 1) / a.splits * step;
-    const int hi = hi64 < len ? (int)hi64 : len;
+    Work w(a, G, step);
+    const int hi = w.hi;
 
     // The query, scaled, this lane's elements.
     float q[G][EL], acc[G][EL], m[G], l[G];
@@ -118,15 +236,14 @@ __global__ void __launch_bounds__(kThreads) k_paged_attention(AttnArgs a) {
 #pragma unroll
             for (int e = 0; e < EV; ++e) {
                 const int i = (v * VL + vl) * EV + e;
-                q[g][v * EV + e] = g < heads && i < hd
-                    ? load_elem(a.q, a.q_type, (int64_t)row * a.q_stride + (int64_t)(head0 + g) * hd + i) * a.scale_log2
+                q[g][v * EV + e] = g < w.heads && i < hd
+                    ? load_elem(a.q, a.q_type, (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd + i) * a.scale_log2
                     : 0.0f;
                 acc[g][v * EV + e] = 0.0f;
             }
     }
-    const bool live = vl * EV < hd;  // VPL > 1 only where every vector of every lane is tested below
-    const char* kbase = static_cast<const char*>(a.ck) + ((int64_t)kvh * hd + vl * EV) * sizeof(TC);
-    const char* vbase = static_cast<const char*>(a.cv) + ((int64_t)kvh * hd + vl * EV) * sizeof(TC);
+    const char* kbase = static_cast<const char*>(a.ck) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
+    const char* vbase = static_cast<const char*>(a.cv) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
     const int64_t row_bytes = a.kv_dim * (int64_t)sizeof(TC);
 
     // Of a tile's keys j * KPL + kg, the lane scores the one whose load index j
@@ -141,44 +258,30 @@ __global__ void __launch_bounds__(kThreads) k_paged_attention(AttnArgs a) {
         for (int b = 0; b < kBits; ++b) r |= ((j >> b) & 1) << (kBits - 1 - b);
         return kg * VL + r;
     };
-    // Cache row of the key this lane scores in the tile at t0; -1: none.
-    auto find = [&](int64_t t0) {
-        const int64_t key = t0 + my_j * KPL + kg;
-        if (key >= hi) return -1;
-        const int blk = (int)key / a.page_size;
-        const int page = __ldg(table + blk);
-        if (page < 0 || page >= a.n_pages) {
-            flags |= CBX_EFLAG_PAGE_OOB;
-            return -1;
-        }
-        return page * a.page_rows + (int)key % a.page_size;
-    };
+    const int my_key = my_j * KPL + kg;  // of a tile, the key this lane scores
 
-    int64_t t0 = lo + (int64_t)warp * TILE;
-    int slot = t0 < hi ? find(t0) : -1;
+    int64_t t0 = w.lo + (int64_t)warp * TILE;
+    int slot = w.find(a, t0 + my_key);
     for (; t0 < hi; t0 += step) {
         uint4 kr[U][VPL], vr[U][VPL];
         int s_of[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) s_of[j] = __shfl_sync(0xffffffffu, slot, lane_of(j));
+        auto load = [&](const char* base, int j, int v) {
+            const bool in = (v * VL + vl) * EV < hd;
+            return s_of[j] >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(base + s_of[j] * row_bytes + v * VL * 16))
+                                      : make_uint4(0, 0, 0, 0);
+        };
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                kr[j][v] = make_uint4(0, 0, 0, 0);
-                if (s_of[j] >= 0 && (VPL == 1 ? live : (v * VL + vl) * EV < hd))
-                    kr[j][v] = __ldg(reinterpret_cast<const uint4*>(kbase + s_of[j] * row_bytes + v * VL * 16));
-            }
+            for (int v = 0; v < VPL; ++v) kr[j][v] = load(kbase, j, v);
 #pragma unroll
         for (int j = 0; j < U; ++j)
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                vr[j][v] = make_uint4(0, 0, 0, 0);
-                if (s_of[j] >= 0 && (VPL == 1 ? live : (v * VL + vl) * EV < hd))
-                    vr[j][v] = __ldg(reinterpret_cast<const uint4*>(vbase + s_of[j] * row_bytes + v * VL * 16));
-            }
+            for (int v = 0; v < VPL; ++v) vr[j][v] = load(vbase, j, v);
         const bool there = slot >= 0;
-        if (t0 + step < hi) slot = find(t0 + step);
+        if (t0 + step < hi) slot = w.find(a, t0 + step + my_key);
         float p[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -248,7 +351,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_attention(AttnArgs a) {
             }
         }
     }
-    if (flags) atomicOr(a.err, flags);
+    if (w.flags) atomicOr(a.err, w.flags);
 
     // Join the warp's key groups, then the CTA's warps.
     const int sf = state_floats(hd);
@@ -278,97 +381,389 @@ __global__ void __launch_bounds__(kThreads) k_paged_attention(AttnArgs a) {
                 }
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * hd; i += kThreads) {
-        const int g = i / hd, e = i % hd;
-        float mm = -INFINITY;
+    finish<kFmaWarps, G>(a, w, smem);
+}
+
+// ---------------------------------------------------------- tensor cores --
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Splits (x, y) into N terms of T, each the rounded rest of those before.
+template <typename T, int N>
+__device__ __forceinline__ void terms_of(float x, float y, uint32_t (&t)[N]) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, smem[(w * G + g) * sf]);
-        float ll = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float* st = smem + (w * G + g) * sf;
-            const float c = rescale(st[0], mm);
-            ll += c * st[1];
-            o += c * st[kStateHead + e];
-        }
-        const int64_t rh = (int64_t)row * a.n_heads + head0 + g;
-        if (a.splits > 1) {
-            float* st = a.part + (rh * a.splits + split) * sf;
-            if (e == 0) {
-                st[0] = mm;
-                st[1] = ll;
-            }
-            st[kStateHead + e] = o;
-        } else {
-            store_elem(a.out, a.q_type, rh * hd + e, len > 0 && ll != 0.0f ? o / ll : 0.0f);
-            if (a.lse && e == 0)
-                a.lse[rh] = ll != 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
-        }
+    for (int i = 0; i < N; ++i) {
+        const float f[2] = {x, y};
+        t[i] = pack32(f, T{});
+        float r[2];
+        unpack32(t[i], r, T{});
+        x -= r[0];
+        y -= r[1];
     }
 }
 
-// Joins the splits' states of one row and head.
-__global__ void __launch_bounds__(128) k_paged_attention_join(AttnArgs a) {
+// 16 bytes to shared memory, zeros where !there.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+}
+
+constexpr int kMmaWarps = 4;
+constexpr int kMmaHeads = 8;   // query heads of a CTA
+constexpr int kMmaTile = 16;   // keys per warp and step
+constexpr int kMmaStages = 3;  // tiles of a warp in shared memory
+
+template <int HD>
+__host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tiles
+    return kMmaStages * 2 * kMmaTile * HD * 2;
+}
+
+// S = Q K^T and O = P V by m16n8k16 products.  Rows 0-7 of the first operand
+// are the first 16-bit term of the 8 heads' values, rows 8-15 the second: Q and
+// P are f32 values written as sums of 16-bit ones, so that the products are as
+// exact as f32 ones where the result is.
+//   QT terms of q: 1 where q has the cache's type; otherwise 3 of bf16 (24 bits)
+//     or 2 of f16 (22 bits; q is brought to [2^10, 2^11) by a power of two, so
+//     that the second term of all but tiny elements is a normal number).
+//   PT terms of p: 2 for a 16-bit result (16 or 22 bits), 3 of bf16 for f32.
+// A third term is a second product on the same accumulators.
+// Each warp streams its own tiles through a ring in shared memory (cp.async, 16
+// bytes a lane, consecutive lanes on consecutive bytes of a key's row), so no
+// CTA barrier stands in the loop, and two tiles are on their way while one is
+// worked on.  Loading the operands' layouts straight from global memory moved
+// the same bytes in 4 times the requests (quarter lines of V): 122 us against
+// 57 us for one row of 65,537 keys, 32 heads over 8 of 128 in bf16 (4.7 TB/s);
+// f32 FMAs with 4 heads a CTA take 107 us there.  The 16-byte vectors of a row are permuted by the
+// row's number, which keeps ldmatrix free of bank conflicts.
+template <typename T, int HD, int QT, int PT>
+__global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
+    constexpr int KS = HD / 16;    // products over the head
+    constexpr int VECS = HD / 8;   // 16-byte vectors of a row in the ring
+    constexpr int step = kMmaTile * kMmaWarps;
+    extern __shared__ __align__(128) float smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int hd = a.head_dim, vecs = hd / 8;
+    grid_dep_wait();
+    grid_dep_launch();
+    Work w(a, kMmaHeads, step);
+
+    // The first operand of S: head g.
+    uint32_t qf[QT][KS][2];
+    float scale = a.scale_log2;
+    {
+        const int64_t base = (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
+        float x[KS][4], most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 16 * s + (e >> 1) * 8 + 2 * t + (e & 1);
+                x[s][e] = g < w.heads && i < hd ? load_elem(a.q, a.q_type, base + i) : 0.0f;
+                most = fmaxf(most, fabsf(x[s][e]));
+            }
+        if constexpr (QT == 2) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            if (most > 0.0f && most < INFINITY) {
+                int e = 264 - (int)(__float_as_uint(most) >> 23);  // biased exponent of the power
+                if (e > 253) e = 253;
+                const float up = __uint_as_float((uint32_t)e << 23);
+                scale *= __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[s][i] *= up;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t f[QT];
+                terms_of<T, QT>(x[s][2 * e], x[s][2 * e + 1], f);
+#pragma unroll
+                for (int k = 0; k < QT; ++k) qf[k][s][e] = f[k];
+            }
+    }
+    float o[VECS][4] = {};
+    float m = -INFINITY, l = 0.0f;  // head g
+    const char* kbase = static_cast<const char*>(a.ck) + (int64_t)w.kvh * hd * 2;
+    const char* vbase = static_cast<const char*>(a.cv) + (int64_t)w.kvh * hd * 2;
+    const int64_t row_bytes = a.kv_dim * 2;
+    constexpr uint32_t kTileBytes = kMmaTile * HD * 2;
+    const uint32_t ring = smem_addr(smem) + warp * mma_ring_bytes<HD>();
+
+    // Puts the tile at t0 in a stage; returns which of its keys are there.
+    auto fetch = [&](int64_t t0, int stage, int slot) {
+        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
+        if (t0 < w.hi) {
+            constexpr int kRows = 32 / VECS;  // rows per instruction
+            const int r0 = lane / VECS, c = lane % VECS;
+            const uint32_t dst = ring + stage * 2 * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kMmaTile / kRows; ++i) {
+                const int r = i * kRows + r0;
+                const int s = __shfl_sync(0xffffffffu, slot, r);
+                const bool in = s >= 0 && c < vecs;
+                const int64_t off = in ? s * row_bytes + c * 16 : 0;
+                const uint32_t at = dst + r * (HD * 2) + ((c ^ (r & 7)) << 4);
+                copy16(at, kbase + off, in);
+                copy16(at + kTileBytes, vbase + off, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return there;
+    };
+
+    const int64_t first = w.lo + (int64_t)warp * kMmaTile;
+    uint64_t there = 0;  // 16 bits for each tile on its way, the oldest on top
+    int slot = w.find(a, first + (lane & 15));
+#pragma unroll
+    for (int s = 0; s < kMmaStages - 1; ++s) {
+        there = there << 16 | fetch(first + s * step, s, slot);
+        slot = w.find(a, first + (int64_t)(s + 1) * step + (lane & 15));
+    }
+    int stage = 0;
+    for (int64_t t0 = first; t0 < w.hi; t0 += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMmaStages - 2) : "memory");
+        __syncwarp();  // all lanes' copies have landed, and all have left the stage that is filled next
+        int next = stage + kMmaStages - 1;
+        if (next >= kMmaStages) next -= kMmaStages;
+        there = there << 16 | fetch(t0 + (int64_t)(kMmaStages - 1) * step, next, slot);
+        slot = w.find(a, t0 + (int64_t)kMmaStages * step + (lane & 15));
+        const uint32_t keys = (uint32_t)(there >> (16 * (kMmaStages - 1))) & 0xffffu;
+        const uint32_t kt = ring + stage * 2 * kTileBytes, vt = kt + kTileBytes;
+        if (++stage == kMmaStages) stage = 0;
+
+        // Scores of head g: keys 2t, 2t + 1 of the first 8, and of the second.
+        float s[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float c[2][4] = {};
+#pragma unroll
+            for (int q = 0; q < KS; q += 2) {
+                uint32_t b[4];
+                ldmatrix4(b, kt + (n * 8 + (lane & 7)) * (HD * 2) + (((2 * q + (lane >> 3)) ^ (lane & 7)) << 4));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    mma16816(c[h], qf[0][q + h][0], QT > 1 ? qf[QT > 1][q + h][0] : 0u, qf[0][q + h][1],
+                             QT > 1 ? qf[QT > 1][q + h][1] : 0u, b[2 * h], b[2 * h + 1], T{});
+                    if constexpr (QT > 2) mma16816(c[h], qf[2][q + h][0], 0u, qf[2][q + h][1], 0u, b[2 * h], b[2 * h + 1], T{});
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float v = c[0][k] + c[1][k];
+                s[2 * n + k] = QT > 1 ? v + (c[0][k + 2] + c[1][k + 2]) : v;
+            }
+        }
+        float best = m;
+        bool in[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            in[i] = keys >> (2 * t + (i & 1) + (i >> 1) * 8) & 1;
+            s[i] = in[i] ? s[i] * scale : -INFINITY;
+            best = fmaxf(best, s[i]);
+        }
+        if (__any_sync(0xffffffffu, best > m)) {
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+            const float c = rescale(m, best);
+            m = best;
+            l *= c;
+#pragma unroll
+            for (int j = 0; j < VECS; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[j][k] *= c;
+        }
+        uint32_t pf[2][PT];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float p0 = in[2 * n] ? ex2_approx(s[2 * n] - m) : 0.0f;
+            const float p1 = in[2 * n + 1] ? ex2_approx(s[2 * n + 1] - m) : 0.0f;
+            l += p0 + p1;
+            terms_of<T, PT>(p0, p1, pf[n]);
+        }
+#pragma unroll
+        for (int j = 0; j < VECS; j += 2) {
+            uint32_t b[4];
+            ldmatrix4_trans(b, vt + (lane & 15) * (HD * 2) + (((j + (lane >> 4)) ^ (lane & 7)) << 4));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mma16816(o[j + h], pf[0][0], pf[0][1], pf[1][0], pf[1][1], b[2 * h], b[2 * h + 1], T{});
+                if constexpr (PT > 2) mma16816(o[j + h], pf[0][2], 0u, pf[1][2], 0u, b[2 * h], b[2 * h + 1], T{});
+            }
+        }
+    }
+    if (w.flags) atomicOr(a.err, w.flags);
+
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the states take the rings' place
+    float* st = smem + (warp * kMmaHeads + g) * state_floats(hd);
+    if (t == 0) {
+        st[0] = m;
+        st[1] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < VECS; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int e = 8 * j + 2 * t + k;
+            if (e < hd) st[kStateHead + e] = o[j][k] + o[j][k + 2];
+        }
+    finish<kMmaWarps, kMmaHeads>(a, w, smem);
+}
+
+// Joins the splits' states of one row and head: first the weight of each split,
+// then the values, whose loads do not depend on one another.
+constexpr int kJoinThreads = 64;
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttnArgs a) {
+    __shared__ float weight[kMaxSplits];
     grid_dep_wait();
     grid_dep_launch();
     const int64_t rh = blockIdx.x;
-    const int sf = state_floats(a.head_dim);
+    const int sf = state_floats(a.head_dim), lane = threadIdx.x & 31;
     const float* st = a.part + rh * a.splits * sf;
-    float mm = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, st[s * sf]);
-    float ll = 0.0f;
-    for (int s = 0; s < a.splits; ++s) ll += rescale(st[s * sf], mm) * st[s * sf + 1];
-    for (int e = threadIdx.x; e < a.head_dim; e += 128) {
-        float o = 0.0f;
-        for (int s = 0; s < a.splits; ++s) o += rescale(st[s * sf], mm) * st[s * sf + kStateHead + e];
-        store_elem(a.out, a.q_type, rh * a.head_dim + e, ll != 0.0f ? o / ll : 0.0f);
+    // every warp for itself: kMaxSplits / 32 splits a lane
+    float m[kMaxSplits / 32], l[kMaxSplits / 32], mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+        const int s = i * 32 + lane;
+        m[i] = s < a.splits ? st[s * sf] : -INFINITY;
+        l[i] = s < a.splits ? st[s * sf + 1] : 0.0f;
+        mm = fmaxf(mm, m[i]);
     }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[rh] = ll != 0.0f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; ++i) {
+        const float c = rescale(m[i], mm);
+        ll += c * l[i];
+        if (threadIdx.x < 32) weight[i * 32 + lane] = c;
+    }
+    ll = warp_sum(ll);
+    __syncthreads();
+    const float r = ll != 0.0f ? 1.0f / ll : 0.0f;
+    for (int e = threadIdx.x; e < a.head_dim; e += kJoinThreads) {
+        float o = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) o = fmaf(weight[s], st[s * sf + kStateHead + e], o);
+        store_elem(a.out, a.q_type, rh * a.head_dim + e, o * r);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[rh] = lse_of(mm, ll);
 }
 
+// Query heads of a CTA.
 int group_chunk(int group) { return group >= 3 ? 4 : group; }
-
-int choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t max_keys) {
-    const int gc = group_chunk(group);
-    const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
-    int64_t s = (2 * num_sms() + ctas - 1) / ctas;
-    const int64_t most = max_keys / kMinKeys;
-    if (s > most) s = most;
-    if (s > kMaxSplits) s = kMaxSplits;
-    return s < 1 ? 1 : (int)s;
+bool use_mma(int cache_type, int group, int head_dim) {
+    return cache_type != CBX_TYPE_F32 && group > 1 && head_dim <= 128;
 }
 
-template <typename TC, int VL, int VPL, int G>
-int run_attention(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
-    const size_t smem = sizeof(float) * kWarps * G * state_floats(a.head_dim);
-    auto kern = k_paged_attention<TC, VL, VPL, G>;
+struct Splits {
+    int n;
+    bool cluster;
+};
+// CTAs over the keys of a row.  The host knows only the longest length the block
+// table can hold, so the cost is that of rows of that length, in keys: waves of
+// resident CTAs, each its whole steps and about 512 keys' time of start and end;
+// joining in a cluster costs little, over the workspace a second launch.
+// Measured in us (B200), splits 1 / 4 / 8 in a cluster, 16 / 32 / 48 over the
+// workspace:
+//   1 row, 1000 keys, 16 kv heads of 64, f32     9.6 / 5.5 / 5.0, 10.0 / 14.7 / 23.4
+//   1 row, 65,537 keys, 8 kv heads of 128, bf16  708 / - / 98, 60 / 57 / 77
+//   64 rows up to 2048, 16 kv heads of 64, f16   56 / 105 / 182
+// (Clusters of 16 were no faster than 16 splits over the workspace: 65 us.)
+Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, int cache_type,
+                     int64_t max_keys) {
+    const bool mma = use_mma(cache_type, group, (int)head_dim);
+    const int gc = mma ? kMmaHeads : group_chunk(group);
+    const int64_t vecs = head_dim * type_size(cache_type) / 16;
+    const int64_t step = mma ? kMmaTile * kMmaWarps
+                       : kFmaWarps * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
+    const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? 4 : 2);
+    const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
+    const int64_t steps = (max_keys + step - 1) / step;
+    int64_t least = 0, best = 1;
+    for (int64_t n = 1; n <= (max_keys >= 8192 ? kMaxSplits : kMaxCluster) && n <= steps; ++n) {
+        const int64_t waves = (ctas * n + resident - 1) / resident;
+        const int64_t cost = waves * ((steps + n - 1) / n * step + 512) +
+                             (n == 1 ? 0 : n <= kMaxCluster ? 256 : 512 + 24 * n);
+        if (n == 1 || cost < least) {
+            least = cost;
+            best = n;
+        }
+    }
+    return {(int)best, best > 1 && best <= kMaxCluster};
+}
+
+cudaError_t launch_attend(void (*kern)(AttnArgs), int warps, size_t smem, const AttnArgs& a,
+                          int64_t n_rows, cudaStream_t st) {
     const dim3 grid((unsigned)a.splits, (unsigned)(a.n_kv * a.chunks), (unsigned)n_rows);
-    cudaError_t e = launch(kern, grid, dim3(kThreads), smem, st, a);
+    if (a.cluster) return launch_cluster(kern, grid, dim3(warps * 32), smem, (unsigned)a.splits, st, a);
+    cudaError_t e = launch(kern, grid, dim3(warps * 32), smem, st, a);
     if (e == cudaSuccess && a.splits > 1)
-        e = launch(k_paged_attention_join, dim3((unsigned)(n_rows * a.n_heads)), dim3(128), 0, st, a);
-    return launch_status(e, "cbx_paged_decode_attention");
+        e = launch(k_attend_join, dim3((unsigned)(n_rows * a.n_heads)), dim3(kJoinThreads), 0, st, a);
+    return e;
 }
 
 template <typename TC, int VL, int VPL>
-int run_group(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
-    switch (group_chunk(a.group)) {
-        case 1: return run_attention<TC, VL, VPL, 1>(a, n_rows, st);
-        case 2: return run_attention<TC, VL, VPL, 2>(a, n_rows, st);
-        default: return run_attention<TC, VL, VPL, 4>(a, n_rows, st);
-    }
+cudaError_t run_fma(AttnArgs a, int64_t n_rows, cudaStream_t st) {
+    const int gc = group_chunk(a.group);
+    a.chunks = (a.group + gc - 1) / gc;
+    const size_t smem = sizeof(float) * (kFmaWarps + 1) * gc * state_floats(a.head_dim);
+    void (*kern)(AttnArgs) = gc == 1 ? k_attend_fma<TC, VL, VPL, 1>
+                           : gc == 2 ? k_attend_fma<TC, VL, VPL, 2> : k_attend_fma<TC, VL, VPL, 4>;
+    return launch_attend(kern, kFmaWarps, smem, a, n_rows, st);
+}
+
+template <typename T, int HD>
+cudaError_t run_mma(AttnArgs a, int64_t n_rows, bool same_type, cudaStream_t st) {
+    constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+    a.chunks = (a.group + kMmaHeads - 1) / kMmaHeads;
+    const size_t states = sizeof(float) * (kMmaWarps + 1) * kMmaHeads * state_floats(a.head_dim);
+    const size_t rings = (size_t)kMmaWarps * mma_ring_bytes<HD>();
+    const size_t smem = states > rings ? states : rings;
+    void (*kern)(AttnArgs) = same_type ? k_attend_mma<T, HD, 1, 2> : k_attend_mma<T, HD, bf16 ? 3 : 2, bf16 ? 3 : 2>;
+    if (smem > 48 * 1024 && !smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
+    return launch_attend(kern, kMmaWarps, smem, a, n_rows, st);
 }
 
 template <typename TC>
-int run_head(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
+cudaError_t run_head(const AttnArgs& a, int cache_type, int64_t n_rows, cudaStream_t st) {
+    if constexpr (sizeof(TC) == 2) {
+        if (use_mma(cache_type, a.group, a.head_dim))
+            return a.head_dim <= 64 ? run_mma<TC, 64>(a, n_rows, a.q_type == cache_type, st)
+                                    : run_mma<TC, 128>(a, n_rows, a.q_type == cache_type, st);
+    }
     const int vecs = (a.head_dim + Vec<TC>::n - 1) / Vec<TC>::n;
-    if (vecs <= 4) return run_group<TC, 4, 1>(a, n_rows, st);
-    if (vecs <= 8) return run_group<TC, 8, 1>(a, n_rows, st);
-    if (vecs <= 16) return run_group<TC, 16, 1>(a, n_rows, st);
-    if (vecs <= 32) return run_group<TC, 32, 1>(a, n_rows, st);
-    if constexpr (Vec<TC>::n == 4) return run_group<TC, 32, 2>(a, n_rows, st);
-    return fail(CBX_ERR_INVALID_ARG, "cbx_paged_decode_attention: head_dim %d", a.head_dim);
+    if (vecs <= 4) return run_fma<TC, 4, 1>(a, n_rows, st);
+    if (vecs <= 8) return run_fma<TC, 8, 1>(a, n_rows, st);
+    if (vecs <= 16) return run_fma<TC, 16, 1>(a, n_rows, st);
+    if constexpr (sizeof(TC) == 4)
+        if (vecs > 32) return run_fma<TC, 32, 2>(a, n_rows, st);
+    return run_fma<TC, 32, 1>(a, n_rows, st);
 }
 
 // Sizes that the workspace query and the call check alike.
@@ -391,8 +786,9 @@ int check_sizes(const char* name, int64_t n_rows, int64_t n_heads, int64_t n_kv_
     return CBX_OK;
 }
 
-int64_t workspace_bytes_of(int64_t n_rows, int64_t n_heads, int64_t head_dim, int splits) {
-    return splits > 1 ? n_rows * n_heads * splits * state_floats((int)head_dim) * (int64_t)sizeof(float) : 0;
+int64_t workspace_bytes_of(int64_t n_rows, int64_t n_heads, int64_t head_dim, Splits s) {
+    if (s.n == 1 || s.cluster) return 0;
+    return n_rows * n_heads * s.n * state_floats((int)head_dim) * (int64_t)sizeof(float);
 }
 
 }  // namespace
@@ -408,7 +804,8 @@ extern "C" CBX_API int64_t cbx_paged_decode_attention_workspace(int64_t n_rows, 
     if (rc != CBX_OK) return rc;
     ok();
     if (n_rows == 0) return 0;
-    const int splits = choose_splits(n_rows, n_kv_heads, (int)(n_heads / n_kv_heads), max_blocks * page_size);
+    const Splits splits = choose_splits(n_rows, n_kv_heads, (int)(n_heads / n_kv_heads),
+                                        head_dim, cache_type, max_blocks * page_size);
     return workspace_bytes_of(n_rows, n_heads, head_dim, splits);
 }
 
@@ -449,20 +846,25 @@ extern "C" CBX_API int cbx_paged_decode_attention(
         (page_stride * type_size(cache_type)) % 16)
         return fail(CBX_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);
     const int group = (int)(n_heads / n_kv_heads);
-    const int splits = choose_splits(n_rows, n_kv_heads, group, max_blocks * page_size);
+    const Splits splits = choose_splits(n_rows, n_kv_heads, group, head_dim, cache_type,
+                                        max_blocks * page_size);
     const int64_t need = workspace_bytes_of(n_rows, n_heads, head_dim, splits);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail(CBX_ERR_INVALID_ARG, "%s: workspace of %lld bytes, %lld needed (16-byte aligned)",
                     name, (long long)(workspace ? workspace_bytes : 0), (long long)need);
-    const int gc = group_chunk(group);
-    AttnArgs a{q, q_type, q_row_stride, cache_k, cache_v, (int)n_pages, (int)page_size,
+    int shift = -1;
+    if ((page_size & (page_size - 1)) == 0)
+        for (shift = 0; (int64_t)1 << shift < page_size;) ++shift;
+    AttnArgs a{q, q_type, q_row_stride, cache_k, cache_v, (int)n_pages, (int)page_size, shift,
                (int)(page_stride / kv_dim), kv_dim, table, (int)n_reqs, (int)max_blocks, row_reqs,
-               seq_lens, (int)n_heads, (int)n_kv_heads, group, (int)head_dim, (group + gc - 1) / gc,
-               scale * kLog2e, out, lse, static_cast<float*>(workspace), splits, err_word};
+               seq_lens, (int)n_heads, (int)n_kv_heads, group, (int)head_dim, 1, scale * kLog2e, out,
+               lse, static_cast<float*>(workspace), splits.n, splits.cluster, err_word};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
     switch (cache_type) {
-        case CBX_TYPE_F32: return run_head<float>(a, n_rows, st);
-        case CBX_TYPE_BF16: return run_head<__nv_bfloat16>(a, n_rows, st);
-        default: return run_head<__half>(a, n_rows, st);
+        case CBX_TYPE_F32: e = run_head<float>(a, cache_type, n_rows, st); break;
+        case CBX_TYPE_BF16: e = run_head<__nv_bfloat16>(a, cache_type, n_rows, st); break;
+        default: e = run_head<__half>(a, cache_type, n_rows, st);
     }
+    return launch_status(e, name);
 }

