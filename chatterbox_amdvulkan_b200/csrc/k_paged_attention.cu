@@ -56,10 +56,13 @@ struct AttnArgs {
     int32_t* err;
 };
 
-__device__ __forceinline__ float load_elem(const void* p, int type, int64_t i) {
-    if (type == CBX_TYPE_F32) return static_cast<const float*>(p)[i];
-    if (type == CBX_TYPE_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
-    return to_f(static_cast<const __half*>(p)[i]);
+// Calls f with the query as a pointer of its type: the branch on the type is
+// taken once, not between the loads, which then travel together.
+template <typename F>
+__device__ __forceinline__ void with_type(const void* p, int type, F f) {
+    if (type == CBX_TYPE_F32) f(static_cast<const float*>(p));
+    else if (type == CBX_TYPE_BF16) f(static_cast<const __nv_bfloat16*>(p));
+    else f(static_cast<const __half*>(p));
 }
 __device__ __forceinline__ void store_elem(void* p, int type, int64_t i, float v) {
     if (type == CBX_TYPE_F32) static_cast<float*>(p)[i] = v;
@@ -206,17 +209,39 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Work& w, float* 
     cluster_sync();  // no CTA leaves while another reads its states
 }
 
-constexpr int kFmaWarps = 8;
+// 16 bytes to shared memory, zeros where !there.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
+}
 
-template <typename TC, int VL, int VPL, int G>
-__global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
+// Shape of the FMA kernel.  With one or two query heads, a tile of keys and one
+// of values wait in registers (8 loads each).  With more, the registers belong
+// to the heads, so the loads go through a ring in shared memory, two tiles
+// ahead: each lane copies and reads its own 16-byte cells, so no barrier is
+// needed.
+template <int VL, int VPL, bool RING>
+struct Fma {
+    static constexpr int kWarps = RING ? 4 : 8;
+    static constexpr int kLoads = RING ? 4 : VL < 8 ? VL : 8;  // of keys, and of values, per tile
+    static constexpr int kKeysPerLoad = 32 / VL;
+    static constexpr int kTile = kKeysPerLoad * kLoads;        // keys per warp and step
+    static constexpr int kStep = kTile * kWarps;
+    static constexpr int kStages = 3;
+    static constexpr int kRingBytes = RING ? kStages * 2 * kLoads * VPL * 512 : 0;  // of a warp
+};
+
+template <typename TC, int VL, int VPL, int G, bool RING>
+__global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(AttnArgs a) {
+    using Shape = Fma<VL, VPL, RING>;
     constexpr int EV = Vec<TC>::n;        // elements per 16-byte vector
     constexpr int EL = EV * VPL;          // elements of the head per lane
-    constexpr int U = VL < 8 ? VL : 8;    // loads in flight
-    constexpr int KPL = 32 / VL;          // keys per load
-    constexpr int TILE = KPL * U;         // keys per warp and step
-    constexpr int step = TILE * kFmaWarps;
-    extern __shared__ float smem[];       // states
+    constexpr int U = Shape::kLoads, KPL = Shape::kKeysPerLoad, TILE = Shape::kTile, step = Shape::kStep;
+    extern __shared__ __align__(128) float smem[];  // rings, then states
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vl = lane % VL, kg = lane / VL;
     const int hd = a.head_dim;
@@ -227,20 +252,27 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
 
     // The query, scaled, this lane's elements.
     float q[G][EL], acc[G][EL], m[G], l[G];
+    with_type(a.q, a.q_type, [&](auto* p) {
+        p += (int64_t)w.row * a.q_stride + (int64_t)w.head0 * hd;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int e = 0; e < EV; ++e) {
+                    const int i = (v * VL + vl) * EV + e;
+                    q[g][v * EV + e] = g < w.heads && i < hd ? to_f(p[g * hd + i]) : 0.0f;
+                }
+    });
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         m[g] = -INFINITY;
         l[g] = 0.0f;
 #pragma unroll
-        for (int v = 0; v < VPL; ++v)
-#pragma unroll
-            for (int e = 0; e < EV; ++e) {
-                const int i = (v * VL + vl) * EV + e;
-                q[g][v * EV + e] = g < w.heads && i < hd
-                    ? load_elem(a.q, a.q_type, (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd + i) * a.scale_log2
-                    : 0.0f;
-                acc[g][v * EV + e] = 0.0f;
-            }
+        for (int e = 0; e < EL; ++e) {
+            q[g][e] *= a.scale_log2;
+            acc[g][e] = 0.0f;
+        }
     }
     const char* kbase = static_cast<const char*>(a.ck) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
     const char* vbase = static_cast<const char*>(a.cv) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
@@ -260,28 +292,65 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
     };
     const int my_key = my_j * KPL + kg;  // of a tile, the key this lane scores
 
+    const uint32_t ring = smem_addr(smem) + warp * Shape::kRingBytes + lane * 16;
+    auto cell = [&](int stage, int kv, int j, int v) { return ring + (((stage * 2 + kv) * U + j) * VPL + v) * 512; };
+    // Sends the tile whose keys' rows the lanes hold on its way to a stage.
+    auto fetch = [&](int stage, int rows) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int s = __shfl_sync(0xffffffffu, rows, lane_of(j));
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) {
+                const bool in = s >= 0 && (v * VL + vl) * EV < hd;
+                const int64_t off = in ? s * row_bytes + v * VL * 16 : 0;
+                copy16(cell(stage, 0, j, v), in ? kbase + off : static_cast<const char*>(a.ck), in);
+                copy16(cell(stage, 1, j, v), in ? vbase + off : static_cast<const char*>(a.cv), in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
     int64_t t0 = w.lo + (int64_t)warp * TILE;
-    int slot = w.find(a, t0 + my_key);
+    int slot = w.find(a, t0 + my_key), slot1 = -1, slot2 = -1, stage = 0;  // of this tile and the next two
+    if constexpr (RING) {
+        slot1 = w.find(a, t0 + step + my_key);
+        fetch(0, slot);
+        fetch(1, slot1);
+        slot2 = w.find(a, t0 + 2 * step + my_key);
+    }
     for (; t0 < hi; t0 += step) {
         uint4 kr[U][VPL], vr[U][VPL];
-        int s_of[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) s_of[j] = __shfl_sync(0xffffffffu, slot, lane_of(j));
-        auto load = [&](const char* base, int j, int v) {
-            const bool in = (v * VL + vl) * EV < hd;
-            return s_of[j] >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(base + s_of[j] * row_bytes + v * VL * 16))
-                                      : make_uint4(0, 0, 0, 0);
-        };
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int v = 0; v < VPL; ++v) kr[j][v] = load(kbase, j, v);
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int v = 0; v < VPL; ++v) vr[j][v] = load(vbase, j, v);
         const bool there = slot >= 0;
-        if (t0 + step < hi) slot = w.find(a, t0 + step + my_key);
+        auto landed = [&](int kv, int j, int v) { return lds16(cell(stage, kv, j, v)); };
+        if constexpr (RING) {
+            fetch(stage == 0 ? 2 : stage - 1, slot2);
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) kr[j][v] = landed(0, j, v);
+            slot = slot1;
+            slot1 = slot2;
+            slot2 = w.find(a, t0 + 3 * step + my_key);
+        } else {
+            int s_of[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) s_of[j] = __shfl_sync(0xffffffffu, slot, lane_of(j));
+            auto load = [&](const char* base, int j, int v) {
+                const bool in = (v * VL + vl) * EV < hd;
+                return s_of[j] >= 0 && in ? __ldg(reinterpret_cast<const uint4*>(base + s_of[j] * row_bytes + v * VL * 16))
+                                          : make_uint4(0, 0, 0, 0);
+            };
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) kr[j][v] = load(kbase, j, v);
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int v = 0; v < VPL; ++v) vr[j][v] = load(vbase, j, v);
+            if (t0 + step < hi) slot = w.find(a, t0 + step + my_key);
+        }
         float p[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -336,6 +405,7 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
                 constexpr int kPer32 = 4 / (int)sizeof(TC);
+                if constexpr (RING) vr[j][v] = landed(1, j, v);
                 unpack32(vr[j][v].x, f[v], TC{});
                 unpack32(vr[j][v].y, f[v] + kPer32, TC{});
                 unpack32(vr[j][v].z, f[v] + 2 * kPer32, TC{});
@@ -350,11 +420,16 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
                     for (int e = 0; e < EV; ++e) acc[g][v * EV + e] = fmaf(w, f[v][e], acc[g][v * EV + e]);
             }
         }
+        if (RING) stage = stage == 2 ? 0 : stage + 1;
     }
     if (w.flags) atomicOr(a.err, w.flags);
+    if constexpr (RING) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
 
     // Join the warp's key groups, then the CTA's warps.
     const int sf = state_floats(hd);
+    float* states = smem + Shape::kRingBytes / 4 * Shape::kWarps;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         // each key's p is held by VL / U lanes: count one of them
@@ -366,7 +441,7 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
         for (int e = 0; e < EL; ++e)
 #pragma unroll
             for (int o = VL; o < 32; o <<= 1) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
-        float* st = smem + (warp * G + g) * sf;
+        float* st = states + (warp * G + g) * sf;
         if (lane == 0) {
             st[0] = m[g];
             st[1] = l[g];
@@ -381,7 +456,7 @@ __global__ void __launch_bounds__(kFmaWarps * 32) k_attend_fma(AttnArgs a) {
                 }
         }
     }
-    finish<kFmaWarps, G>(a, w, smem);
+    finish<Shape::kWarps, G>(a, w, states);
 }
 
 // ---------------------------------------------------------- tensor cores --
@@ -415,10 +490,6 @@ __device__ __forceinline__ void terms_of(float x, float y, uint32_t (&t)[N]) {
     }
 }
 
-// 16 bytes to shared memory, zeros where !there.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
@@ -471,16 +542,21 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
     uint32_t qf[QT][KS][2];
     float scale = a.scale_log2;
     {
-        const int64_t base = (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
         float x[KS][4], most = 0.0f;
+        with_type(a.q, a.q_type, [&](auto* p) {
+            p += (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * s + (e >> 1) * 8 + 2 * t + (e & 1);
+                    x[s][e] = g < w.heads && i < hd ? to_f(p[i]) : 0.0f;
+                }
+        });
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 16 * s + (e >> 1) * 8 + 2 * t + (e & 1);
-                x[s][e] = g < w.heads && i < hd ? load_elem(a.q, a.q_type, base + i) : 0.0f;
-                most = fmaxf(most, fabsf(x[s][e]));
-            }
+            for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[s][e]));
         if constexpr (QT == 2) {
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -701,7 +777,7 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
     const int gc = mma ? kMmaHeads : group_chunk(group);
     const int64_t vecs = head_dim * type_size(cache_type) / 16;
     const int64_t step = mma ? kMmaTile * kMmaWarps
-                       : kFmaWarps * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
+                       : 8 * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
     const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? 4 : 2);
     const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
     const int64_t steps = (max_keys + step - 1) / step;
@@ -728,14 +804,28 @@ cudaError_t launch_attend(void (*kern)(AttnArgs), int warps, size_t smem, const 
     return e;
 }
 
+template <typename TC, int VL, int VPL, int G, bool RING>
+cudaError_t run_fma_heads(AttnArgs a, int64_t n_rows, cudaStream_t st) {
+    using Shape = Fma<VL, VPL, RING>;
+    a.chunks = (a.group + G - 1) / G;
+    const size_t smem = sizeof(float) * (Shape::kWarps + 1) * G * state_floats(a.head_dim) +
+                        (size_t)Shape::kRingBytes * Shape::kWarps;
+    auto kern = k_attend_fma<TC, VL, VPL, G, RING>;
+    if (smem > 48 * 1024 && !smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
+    return launch_attend(kern, Shape::kWarps, smem, a, n_rows, st);
+}
+
+// Four query heads take the ring, one and two the registers, in us (B200):
+//   94 rows of 2511 keys, 16 heads over 2 of 64, f32       113 / 169
+//   7 rows of 1922 keys, 32 heads over 16 of 128, f32       46 / 40
+//   128 rows up to 8196 keys, 16 heads of 64, bf16         340 / 312
 template <typename TC, int VL, int VPL>
-cudaError_t run_fma(AttnArgs a, int64_t n_rows, cudaStream_t st) {
-    const int gc = group_chunk(a.group);
-    a.chunks = (a.group + gc - 1) / gc;
-    const size_t smem = sizeof(float) * (kFmaWarps + 1) * gc * state_floats(a.head_dim);
-    void (*kern)(AttnArgs) = gc == 1 ? k_attend_fma<TC, VL, VPL, 1>
-                           : gc == 2 ? k_attend_fma<TC, VL, VPL, 2> : k_attend_fma<TC, VL, VPL, 4>;
-    return launch_attend(kern, kFmaWarps, smem, a, n_rows, st);
+cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
+    switch (group_chunk(a.group)) {
+        case 1: return run_fma_heads<TC, VL, VPL, 1, false>(a, n_rows, st);
+        case 2: return run_fma_heads<TC, VL, VPL, 2, false>(a, n_rows, st);
+        default: return run_fma_heads<TC, VL, VPL, 4, true>(a, n_rows, st);
+    }
 }
 
 template <typename T, int HD>

@@ -600,7 +600,6 @@ def qkv_kv_append(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: torch.T
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _I32, _F32 = torch.int32, torch.float32
-_FNS: dict = {}
 
 
 def _on_device(fn):
@@ -616,14 +615,10 @@ def _on_device(fn):
     return wrapper
 
 
-def _call(fn: str, *args) -> None:
-    """_lib.call with the function looked up once."""
-    f = _FNS.get(fn)
-    if f is None:
-        f = _FNS[fn] = getattr(_lib.load(), fn)
-    status = f(*args)
-    if status != 0:
-        _lib.check(fn, status)
+@functools.cache
+def _fn(name: str):
+    """The library's function, looked up once."""
+    return getattr(_lib.load(), name)
 
 
 def _ok(dev: int, dtype, tensors) -> bool:
@@ -656,7 +651,8 @@ def _refuse_strided(**tensors):
 
 
 def _type_of(t: torch.Tensor) -> int:
-    return _TORCH_TO_CBX[t.dtype] if t.dtype in _TORCH_TO_CBX else _cbx_type(t)
+    v = _TORCH_TO_CBX.get(t.dtype)
+    return _cbx_type(t) if v is None else v
 
 
 def _err_word(err: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
@@ -752,10 +748,13 @@ def paged_plan(seq_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torc
     err = _err_word(err, seq_lens)
     slots, positions, row_reqs, row_lens, row_start, table_o, blocks_o, free_o, n_free_o = [
         t.data_ptr() for t in out]
-    _call("cbx_paged_plan", seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(),
-          n_reqs, max_blocks, int(page_size), n_pages, block_table.data_ptr(), n_blocks.data_ptr(),
-          free_list.data_ptr(), n_free.data_ptr(), table_o, blocks_o, free_o, n_free_o, max_rows,
-          slots, positions, row_reqs, row_lens, row_start, err.data_ptr(), _raw_stream(dev))
+    status = _fn("cbx_paged_plan")(
+        seq_lens.data_ptr(), None if n_new is None else n_new.data_ptr(), n_reqs, max_blocks,
+        int(page_size), n_pages, block_table.data_ptr(), n_blocks.data_ptr(), free_list.data_ptr(),
+        n_free.data_ptr(), table_o, blocks_o, free_o, n_free_o, max_rows, slots, positions,
+        row_reqs, row_lens, row_start, err.data_ptr(), _raw_stream(dev))
+    if status:
+        _lib.check("cbx_paged_plan", status)
     return PagedPlan(*out, err)
 
 
@@ -794,18 +793,24 @@ def qkv_kv_append_paged(qkv: torch.Tensor, bias: torch.Tensor | None, cache_k: t
     dev = qkv.get_device()
     if cache_k.get_device() != dev or cache_v.get_device() != dev or dev < 0:
         _refuse_strided(qkv=qkv, cache_k=cache_k, cache_v=cache_v)
-    if not _ok(dev, _I32, (slots, err)) or not _ok(dev, _F32, (bias,)) or \
-            not _ok(dev, qkv.dtype, (q_out,)):
-        _refuse(_F32, bias=bias) if not _ok(dev, _F32, (bias,)) else None
-        _refuse(qkv.dtype, q_out=q_out) if not _ok(dev, qkv.dtype, (q_out,)) else None
+    if not _ok(dev, _I32, (slots, err)):
         _refuse(_I32, slots=slots, err=err)
-    if q_out is None and with_q:
-        q_out = qkv.new_empty((n_rows, q_dim))
-    err = _err_word(err, qkv)
-    _call("cbx_qkv_kv_append_paged", qkv.data_ptr(), _type_of(qkv), stride,
-          None if bias is None else bias.data_ptr(), n_rows, q_dim, kv_dim, slots.data_ptr(),
-          cache_k.data_ptr(), cache_v.data_ptr(), _type_of(cache_k), P, S, page_stride,
-          None if q_out is None else q_out.data_ptr(), err.data_ptr(), _raw_stream(dev))
+    if bias is not None and not _ok(dev, _F32, (bias,)):
+        _refuse(_F32, bias=bias)
+    if q_out is None:
+        if with_q:
+            q_out = torch.empty((n_rows, q_dim), dtype=qkv.dtype, device=qkv.device)
+    elif not _ok(dev, qkv.dtype, (q_out,)):
+        _refuse(qkv.dtype, q_out=q_out)
+    if err is None or err.numel() != 1:
+        err = _err_word(err, qkv)
+    status = _fn("cbx_qkv_kv_append_paged")(
+        qkv.data_ptr(), _type_of(qkv), stride, None if bias is None else bias.data_ptr(), n_rows,
+        q_dim, kv_dim, slots.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), _type_of(cache_k),
+        P, S, page_stride, None if q_out is None else q_out.data_ptr(), err.data_ptr(),
+        _raw_stream(dev))
+    if status:
+        _lib.check("cbx_qkv_kv_append_paged", status)
     return q_out, err
 
 
@@ -852,7 +857,7 @@ def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torc
     if not _ok(dev, _I32, (block_table, seq_lens, row_reqs, err)):
         _refuse(_I32, block_table=block_table, seq_lens=seq_lens, row_reqs=row_reqs, err=err)
     if out is None:
-        out = q.new_empty((n_rows, H, hd))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif not _ok(dev, q.dtype, (out,)):
         _refuse(q.dtype, out=out)
     lse = torch.empty((n_rows, H), dtype=_F32, device=q.device) if return_lse else None
@@ -865,13 +870,16 @@ def paged_decode_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torc
         elif not _ok(dev, workspace.dtype, (workspace,)):
             _refuse(workspace.dtype, workspace=workspace)
         ws_p, ws_bytes = workspace.data_ptr(), workspace.nbytes
-    err = _err_word(err, q)
-    _call("cbx_paged_decode_attention", q.data_ptr(), _type_of(q), q_stride, cache_k.data_ptr(),
-          cache_v.data_ptr(), ct, P, S, page_stride, block_table.data_ptr(), n_reqs, max_blocks,
-          None if row_reqs is None else row_reqs.data_ptr(), seq_lens.data_ptr(), n_rows, H, Hk,
-          hd, hd ** -0.5 if scale is None else scale, out.data_ptr(),
-          None if lse is None else lse.data_ptr(), ws_p, ws_bytes, err.data_ptr(),
-          _raw_stream(dev))
+    if err is None or err.numel() != 1:
+        err = _err_word(err, q)
+    status = _fn("cbx_paged_decode_attention")(
+        q.data_ptr(), _type_of(q), q_stride, cache_k.data_ptr(), cache_v.data_ptr(), ct, P, S,
+        page_stride, block_table.data_ptr(), n_reqs, max_blocks,
+        None if row_reqs is None else row_reqs.data_ptr(), seq_lens.data_ptr(), n_rows, H, Hk, hd,
+        hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        None if lse is None else lse.data_ptr(), ws_p, ws_bytes, err.data_ptr(), _raw_stream(dev))
+    if status:
+        _lib.check("cbx_paged_decode_attention", status)
     return (out, lse) if return_lse else out
 
 
@@ -924,21 +932,26 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top_k: int
             raise ValueError(f"logits' rows overlap: stride {stride} < {vocab}")
     if not 0 <= top_k <= vocab or top_k > _lib.LOGPROBS_MAX_TOP:
         raise ValueError(f"top_k {top_k} outside [0, min(vocab, {_lib.LOGPROBS_MAX_TOP})]")
-    if tokens is not None and tokens.numel() != n_rows:
-        raise ValueError(f"tokens has {tokens.numel()} entries for {n_rows} rows")
+    if tokens is not None and tokens.shape != (n_rows,):
+        raise ValueError(f"tokens has shape {tuple(tokens.shape)}, not one entry for each of {n_rows} rows")
     dev = logits.get_device()
     if dev < 0:
         _refuse_strided(logits=logits)
     if not _ok(dev, _I32, (tokens, err)):
         _refuse(_I32, tokens=tokens, err=err)
-    device = logits.device
-    entropy = torch.empty(n_rows, dtype=_F32, device=device)
-    lp = torch.empty_like(entropy) if tokens is not None else None
-    top = torch.empty((n_rows, top_k), dtype=_F32, device=device)
+    if tokens is not None:
+        lp = torch.empty_like(tokens, dtype=_F32)
+        entropy = torch.empty_like(lp)
+    else:
+        lp, entropy = None, torch.empty(n_rows, dtype=_F32, device=logits.device)
+    top = torch.empty((n_rows, top_k), dtype=_F32, device=logits.device)
     ids = torch.empty_like(top, dtype=_I32)
-    err = _err_word(err, logits)
-    _call("cbx_token_logprobs", logits.data_ptr(), _type_of(logits), stride, n_rows, vocab,
-          None if tokens is None else tokens.data_ptr(), top_k,
-          None if lp is None else lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
-          top.data_ptr(), err.data_ptr(), _raw_stream(dev))
+    if err is None or err.numel() != 1:
+        err = _err_word(err, logits)
+    status = _fn("cbx_token_logprobs")(
+        logits.data_ptr(), _type_of(logits), stride, n_rows, vocab,
+        None if lp is None else tokens.data_ptr(), top_k, None if lp is None else lp.data_ptr(),
+        entropy.data_ptr(), ids.data_ptr(), top.data_ptr(), err.data_ptr(), _raw_stream(dev))
+    if status:
+        _lib.check("cbx_token_logprobs", status)
     return TokenLogprobs(lp, entropy, ids, top, err)
