@@ -29,6 +29,8 @@
 // Bound by HBM at many rows (each logit is read once), by latency at few: NT
 // threads share a row, from a warp each (no barriers; the work per row outside
 // the loop is that of one warp) to a CTA of 512.
+#include <type_traits>
+
 #include "cbx_common.cuh"
 
 namespace cbx {
@@ -96,7 +98,7 @@ struct Stat {
 constexpr float kSlack = 8.0f;
 
 // Adds N values (N even) whose maximum is b.  NaN and +inf make s a NaN or inf.
-template <int N>
+template <int N, bool BOUNDED>
 __device__ __forceinline__ void add(Stat& st, const float2 (&f)[N / 2], float b) {
     const float to = reference_of(b);
     if (to > st.r + kSlack) st.raise(to);
@@ -106,7 +108,9 @@ __device__ __forceinline__ void add(Stat& st, const float2 (&f)[N / 2], float b)
         const float2 d = __ffma2_rn(f[i], pair(kLog2e), ref);
         const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
         st.s = __fadd2_rn(st.s, e);
-        st.t = __ffma2_rn(e, make_float2(fmaxf(d.x, kLeast), fmaxf(d.y, kLeast)), st.t);
+        // 0 * -inf would be NaN; 16-bit values come bounded from widen()
+        if constexpr (BOUNDED) st.t = __ffma2_rn(e, d, st.t);
+        else st.t = __ffma2_rn(e, make_float2(fmaxf(d.x, kLeast), fmaxf(d.y, kLeast)), st.t);
     }
 }
 
@@ -131,8 +135,29 @@ struct Row {
     }
 };
 
+// The least maximum whose row the sums above are right for: far enough above
+// what widen() raises -inf to that this weighs nothing.
 template <typename T>
+__device__ __forceinline__ float least_max() {
+    return sizeof(T) == 4 ? -kHuge : __is_same(T, __half) ? -65000.0f : -1e29f;
+}
+
+// Elements of a vector as f32.  With BOUNDED, 16-bit ones are raised to -1e30
+// (bf16) or the lowest finite value (f16), two in one instruction: no weight
+// beside a maximum of least_max or more, but a finite x log2 e.  NaN stays.
+template <typename T, bool BOUNDED>
 __device__ __forceinline__ void widen(uint4 w, float2 (&f)[Vec<T>::n / 2]) {
+    if constexpr (BOUNDED && sizeof(T) == 2) {
+        constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+        using T2 = std::conditional_t<bf16, __nv_bfloat162, __half2>;
+        const float low[2] = {bf16 ? -1e30f : -65504.0f, bf16 ? -1e30f : -65504.0f};
+        const uint32_t b = pack32(low, T{});
+        auto raise = [&](uint32_t v) {
+            const T2 r = __hmax2_nan(*reinterpret_cast<const T2*>(&v), *reinterpret_cast<const T2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        };
+        w = make_uint4(raise(w.x), raise(w.y), raise(w.z), raise(w.w));
+    }
     float g[Vec<T>::n];
     constexpr int k = 4 / (int)sizeof(T);
     unpack32(w.x, g, T{});
@@ -296,6 +321,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
     const int64_t stride = (int64_t)gridDim.x * kTeams;
     const int64_t r0 = (int64_t)blockIdx.x * kTeams + threadIdx.x / NT;
     constexpr int kUnroll = Tm::kUnroll;
+    constexpr bool kBounded = sizeof(T) == 2;
     constexpr int kBatch = NT * kUnroll;  // vectors that the team takes at a time
     // A row's b-th batch; behind the row: nothing.
     auto fetch = [&](const Row<T>& row, int b, uint4 (&w)[kUnroll]) {
@@ -350,15 +376,15 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
                 float2 f[kUnroll * EV / 2];
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
-                    widen<T>(w[u], *reinterpret_cast<float2(*)[EV / 2]>(f + u * EV / 2));
-                add<kUnroll * EV>(st, f, m);
+                    widen<T, kBounded>(w[u], *reinterpret_cast<float2(*)[EV / 2]>(f + u * EV / 2));
+                add<kUnroll * EV, kBounded>(st, f, m);
             } else {
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
                     if (b * kBatch + u * NT < row.nv) {
                         float2 f[EV / 2];
-                        widen<T>(w[u], f);
-                        add<EV>(st, f, m);
+                        widen<T, kBounded>(w[u], f);
+                        add<EV, kBounded>(st, f, m);
                     }
             }
             if (TOP) {
@@ -374,42 +400,80 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
         float2 ends[1] = {{to_f(end_head), to_f(end_tail)}};
         if (tid < row.head || tid < row.V - row.tail) {
             const float m = fmaxf(ends[0].x, ends[0].y);
-            add<2>(st, ends, m);
+            add<2, false>(st, ends, m);
             top = fmaxf(top, m);
         }
 
-        // Maximum of the row, then the sums relative to its reference.
-        float m = warp_max(top);
+        // Maximum of the row, and of the 32 groups.
+        float m = warp_max(top), group = top;
+        if (TOP && tid == 0) sh.count = 0;
         if constexpr (NT > 32) {
-            float g = top;
 #pragma unroll
-            for (int o = 1; o < NT / 32; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-            if (tid % (NT / 32) == 0) sh.group[tid / (NT / 32)] = g;
-            if (TOP && tid == 0) sh.count = 0;
+            for (int o = 1; o < NT / 32; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+            if (tid % (NT / 32) == 0) sh.group[tid / (NT / 32)] = group;
             __syncthreads();
-            m = warp_max(sh.group[lane]);
+            group = sh.group[lane];
+            m = warp_max(group);
+        } else if (TOP) {
+            __syncwarp();
         }
-        float ref = reference_of(m);
+        // The sums relative to the row's reference.
+        const float ref = reference_of(m);
         st.raise(ref);
         float s = warp_sum(st.s.x + st.s.y), t = warp_sum(st.t.x + st.t.y);
-        if constexpr (NT > 32) {
-            if (lane == 0) {
-                sh.s[warp] = s;
-                sh.t[warp] = t;
+        if (NT > 32 && lane == 0) {
+            sh.s[warp] = s;
+            sh.t[warp] = t;
+        }
+        if constexpr (TOP) {
+            float tau = m;
+            if (a.top_k > 1) tau = __shfl_sync(0xffffffffu, sort_falling(group, lane), a.top_k - 1);
+            if (top >= tau && (tau != -INFINITY || row.V <= Tm::kCap)) {
+                auto put = [&](int at, float v, int j) {
+                    if (at < Tm::kCap) sh.list[at] = key_of(v, j);
+                };
+                if (tid < row.head && ends[0].x >= tau) put(atomicAdd(&sh.count, 1), ends[0].x, tid);
+                if (tid < row.V - row.tail && ends[0].y >= tau) put(atomicAdd(&sh.count, 1), ends[0].y, row.tail + tid);
+                uint32_t todo = 0;
+                for (int q = 0; q < n_segs; ++q) todo |= (sh.seg[q * NT + tid] >= tau ? 1u : 0u) << q;
+                for (; todo; todo &= todo - 1) {
+                    const int b0 = (__ffs(todo) - 1) * per;
+                    for (int b = b0; b < b0 + per && b < batches; ++b) {
+                        uint4 w[kUnroll];
+                        fetch(row, b, w);
+#pragma unroll
+                        for (int u = 0; u < kUnroll; ++u) {
+                            const uint4 one[1] = {w[u]};
+                            if (b * kBatch + u * NT + tid >= row.nv || max_of(one, T{}) < tau) continue;
+                            float2 f[EV / 2];
+                            widen<T, false>(w[u], f);
+                            int n = 0;
+#pragma unroll
+                            for (int e = 0; e < EV / 2; ++e) n += (f[e].x >= tau) + (f[e].y >= tau);
+                            if (!n) continue;  // all NaN
+                            int at = atomicAdd(&sh.count, n);
+                            const int j = row.first(b * kBatch + u * NT + tid);
+#pragma unroll
+                            for (int e = 0; e < EV / 2; ++e) {
+                                if (f[e].x >= tau) put(at++, f[e].x, j + 2 * e);
+                                if (f[e].y >= tau) put(at++, f[e].y, j + 2 * e + 1);
+                            }
+                        }
+                    }
+                }
             }
-            __syncthreads();
+        }
+        if (NT > 32 || TOP) Tm::sync();
+        if constexpr (NT > 32) {
             s = t = 0.0f;
 #pragma unroll
             for (int w = 0; w < Tm::kWarps; ++w) {
                 s += sh.s[w];
                 t += sh.t[w];
             }
-        } else if (TOP) {
-            if (lane == 0) sh.count = 0;
-            __syncwarp();
         }
         bool bad = false, huge = false;
-        if (!(fabsf(m) <= kHuge && s <= 3e38f)) {  // rare: no distribution, or logits near the type's limits
+        if (!(m >= least_max<T>() && m <= kHuge && s <= 3e38f)) {  // rare: no distribution, or logits near the type's limits
             huge = true;
             sums_from_differences<T, NT>(row, tid, m, sh, &s, &t);
             bad = fabsf(m) == INFINITY || s != s;
@@ -426,44 +490,8 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
             }
         }
         if constexpr (TOP) {
-            float tau = m;
-            if (a.top_k > 1)
-                tau = __shfl_sync(0xffffffffu, sort_falling(NT > 32 ? sh.group[lane] : top, lane), a.top_k - 1);
-            // Puts the elements of the mask, first + bit, on the list.
-            auto offer = [&](uint32_t mask, int first) {
-                if (!mask) return;
-                int at = atomicAdd(&sh.count, __popc(mask));
-                for (; mask; mask &= mask - 1, ++at) {
-                    const int j = first + __ffs(mask) - 1;
-                    if (at < Tm::kCap) sh.list[at] = key_of(to_f(row.x[j]), j);
-                }
-            };
-            if (!bad && top >= tau && (tau != -INFINITY || row.V <= Tm::kCap)) {
-                if (tid < row.head) offer(ends[0].x >= tau, tid);
-                if (tid < row.V - row.tail) offer(ends[0].y >= tau, row.tail + tid);
-                uint32_t todo = 0;
-                for (int q = 0; q < n_segs; ++q) todo |= (sh.seg[q * NT + tid] >= tau ? 1u : 0u) << q;
-                while (todo) {
-                    int i = (__ffs(todo) - 1) * per * kUnroll;
-                    todo &= todo - 1;
-                    for (const int i1 = i + per * kUnroll; i < i1; ++i) {
-                        const int v = tid + i * NT;
-                        if (v >= row.nv) break;
-                        const uint4 w[1] = {row.vec(v)};
-                        if (max_of(w, T{}) < tau) continue;
-                        float2 f[EV / 2];
-                        widen<T>(w[0], f);
-                        uint32_t mask = 0;
-#pragma unroll
-                        for (int e = 0; e < EV / 2; ++e)
-                            mask |= (f[e].x >= tau ? 1u : 0u) << (2 * e) | (f[e].y >= tau ? 2u : 0u) << (2 * e);
-                        offer(mask, row.first(v));
-                    }
-                }
-            }
-            Tm::sync();
             const int n = sh.count;
-            if (n >= a.top_k && n <= Tm::kCap) {
+            if (!bad && n >= a.top_k && n <= Tm::kCap) {
                 for (int i = tid; i < n; i += NT) {
                     const unsigned long long key = sh.list[i];
                     int rank = 0;
@@ -510,15 +538,17 @@ int run_team(const LogprobArgs& a, cudaStream_t st) {
 //   2048 x 50276 f16    110.2 / 53.6 / 62.7 / 111.8
 //   4200 x 20000 bf16    66.8 / 57.5 / 61.6 / 131.4
 //   8192 x 6563 bf16     29.0 / 46.1 / 65.4 / 160.9
+// A row with less than a vector for each thread would leave groups without a
+// maximum and so without a bound for its alternatives: it takes fewer threads.
 // The warp's list holds the candidates of up to 24 alternatives (about 32 ln(1 /
 // (1 - k / 32)) of them, 44 for 24).
 template <typename T>
 int run_logprobs(const LogprobArgs& a, cudaStream_t st) {
-    const int64_t rows = a.n_rows, sms = num_sms();
-    const bool is_short = a.vocab <= 2048 * Vec<T>::n;  // up to 32 KB
-    if (rows <= sms) return run_team<T, 512>(a, st);
-    if (rows >= 7 * sms && is_short && a.top_k <= 24) return run_team<T, 32>(a, st);
-    if (rows >= 10 * sms) return run_team<T, 128>(a, st);
+    const int64_t rows = a.n_rows, sms = num_sms(), vecs = a.vocab / Vec<T>::n;
+    const bool warp = a.top_k <= 24;
+    if (warp && (vecs < 128 || (rows >= 7 * sms && vecs <= 2048))) return run_team<T, 32>(a, st);
+    if (rows <= sms && vecs >= 512) return run_team<T, 512>(a, st);
+    if (rows >= 10 * sms || vecs < 256) return run_team<T, 128>(a, st);
     return run_team<T, 256>(a, st);
 }
 

@@ -111,6 +111,22 @@ def test_logprobs_masked_rows(ops, t):
     assert got.logprobs[2] == -math.inf and abs(got.logprobs[4].item() + math.log(V)) < 1e-5
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V", [50, 1000, 6563])
+def test_logprobs_largest_near_the_types_lowest(ops, t, V):
+    """Rows whose largest logit is itself a mask value, beside -inf and other mask values."""
+    low = torch.finfo(t).min
+    x = torch.full((5, V), -math.inf, device="cuda", dtype=t)
+    x[0, ::3] = low
+    x[1] = low
+    x[2, 1::2] = -1e30 if t != torch.float16 else -65000.0
+    x[3, ::2], x[3, 5] = low, low / 2
+    x[4], x[4, 7] = -60000.0, 3.0
+    tokens = torch.tensor([3, 5, 1, 5, 7], dtype=torch.int32, device="cuda")
+    for k in (1, 6):
+        check(ops.token_logprobs(x, tokens, top_k=k), x, tokens, k)
+
+
 def test_logprobs_rows_without_a_distribution(ops):
     """Nothing but -inf, a +inf, a NaN: values NaN; the order of the alternatives still holds."""
     x = torch.randn(4, 500, device="cuda")
