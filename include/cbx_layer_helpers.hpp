@@ -22,6 +22,9 @@
 //   cbx::get_rows_add_batched  the same for B utterances at positions n_past + t
 //   cbx::t3_prefill_input    t3.cpp:428-455 ([cond ; speech[prompt] ; tokens] + positions)
 //   cbx::qkv_kv_append       t3.cpp:465-489 (qkv bias, Q, K / V cache writes)
+//   cbx::paged_plan, qkv_kv_append_paged, paged_decode_attention, token_logprobs:
+//                            a decode step on a paged KV cache (t3.cpp:465-528 and
+//                            the logits of :612-614, for many requests at once)
 //   cbx::generate_source     hift_vocoder.cpp:853-965 (HiFTVocoder::generate_source)
 //   cbx::engine_source_draws hift_vocoder.cpp:889-913 (its std::mt19937 draws, host)
 //   cbx::stft_centered       hift_vocoder.cpp:465-498 (+ s_stft rows, :627-638)
@@ -352,6 +355,137 @@ inline Tensor* qkv_kv_append(const Tensor& qkv, const Tensor* qkv_b, Tensor& cac
                           max_context, q_out ? static_cast<float*>(q_out->data) : nullptr,
                           err_word, stream),
         ret);
+}
+
+// State of a paged KV cache, all int32 on the device: block_table ne =
+// (max_blocks, n_reqs), n_blocks ne = (n_reqs), free_list ne = (n_pages), n_free
+// ne = (1).  Initially: block_table -1, n_blocks 0, free_list 0 .. n_pages - 1,
+// n_free n_pages.
+struct PagedState {
+    Tensor block_table, n_blocks, free_list, n_free;
+};
+
+// One step's rows and the state after it, updated in place: seq_lens int32 ne =
+// (n_reqs) (tokens each request holds after the step, 0: it ended), n_new int32
+// ne = (n_reqs) or null (one token each); slots, positions, row_reqs, row_lens
+// int32 ne = (max_rows), the last two may be null.
+inline Tensor* paged_plan(const Tensor& seq_lens, const Tensor* n_new, PagedState& st,
+                          int64_t page_size, Tensor& slots, Tensor& positions, Tensor* row_reqs,
+                          Tensor* row_lens, int32_t* err_word, cbx_stream_t stream = nullptr) {
+    auto i32 = [](const Tensor* t) { return t ? static_cast<int32_t*>(t->data) : nullptr; };
+    const int64_t n_reqs = nelements(seq_lens), rows = nelements(slots);
+    if (st.block_table.ne[1] != n_reqs || nelements(st.n_blocks) != n_reqs ||
+        nelements(st.n_free) != 1 || (n_new && nelements(*n_new) != n_reqs) ||
+        nelements(positions) != rows || (row_reqs && nelements(*row_reqs) != rows) ||
+        (row_lens && nelements(*row_lens) != rows)) {
+        std::fprintf(stderr, "paged_plan: state and rows of unequal sizes\n");
+        return nullptr;
+    }
+    return detail::report(
+        "paged_plan",
+        cbx_paged_plan(i32(&seq_lens), i32(n_new), n_reqs, st.block_table.ne[0], page_size,
+                       nelements(st.free_list), i32(&st.block_table), i32(&st.n_blocks),
+                       i32(&st.free_list), i32(&st.n_free), i32(&st.block_table),
+                       i32(&st.n_blocks), i32(&st.free_list), i32(&st.n_free), rows, i32(&slots),
+                       i32(&positions), i32(row_reqs), i32(row_lens), nullptr, err_word, stream),
+        &slots);
+}
+
+namespace detail {
+// A paged cache: ne = (kv_dim, page_size, n_pages), rows and pages dense or the
+// pages further apart (one layer of a pool).  Returns the page stride in elements.
+inline bool paged_cache(const Tensor& k, const Tensor& v, int64_t* page_stride) {
+    const size_t s = type_size(k.type);
+    if (k.type != v.type || k.ne[3] != 1) return false;
+    for (int i = 0; i < 3; ++i)
+        if (k.ne[i] != v.ne[i] || (k.ne[i] > 1 && k.nb[i] != v.nb[i])) return false;
+    if (k.nb[0] != s || k.nb[1] != s * (size_t)k.ne[0] || k.nb[2] % s) return false;
+    *page_stride = (int64_t)(k.nb[2] / s);
+    return true;
+}
+}  // namespace detail
+
+// t3.cpp:465-489 on a paged cache: qkv ne = (q_dim + 2 kv_dim, N) f32 / f16 /
+// bf16, qkv_b f32 or null, caches ne = (kv_dim, page_size, n_pages), slots int32
+// ne = (N), q_out ne = (q_dim, N) of qkv's type or null.
+inline Tensor* qkv_kv_append_paged(const Tensor& qkv, const Tensor* qkv_b, Tensor& cache_k,
+                                   Tensor& cache_v, const Tensor& slots, Tensor* q_out,
+                                   int32_t* err_word, cbx_stream_t stream = nullptr) {
+    int64_t sx = 0, ps = 0;
+    const int64_t kv = cache_k.ne[0], qd = qkv.ne[0] - 2 * kv;
+    if (!detail::uniform_rows(qkv, &sx) || !detail::paged_cache(cache_k, cache_v, &ps) || qd < 0 ||
+        nelements(slots) < nrows(qkv) || (qkv_b && nelements(*qkv_b) != qkv.ne[0]) ||
+        (q_out && (q_out->type != qkv.type || !detail::contiguous(*q_out) ||
+                   nelements(*q_out) != qd * nrows(qkv)))) {
+        std::fprintf(stderr, "qkv_kv_append_paged: rows of q_dim + 2 kv_dim and paged caches of one type\n");
+        return nullptr;
+    }
+    return detail::report(
+        "qkv_kv_append_paged",
+        cbx_qkv_kv_append_paged(qkv.data, qkv.type, sx, detail::f32_or_null(qkv_b), nrows(qkv), qd,
+                                kv, static_cast<const int32_t*>(slots.data), cache_k.data,
+                                cache_v.data, cache_k.type, cache_k.ne[2], cache_k.ne[1], ps,
+                                q_out ? q_out->data : nullptr, err_word, stream),
+        q_out ? q_out : &cache_k);
+}
+
+// Attention of one new token per row (what the engine's graph computes for one
+// query between t3.cpp:489 and :528): q, out ne = (head_dim, n_heads, N) of one
+// type; caches as above; block_table int32 ne = (max_blocks, n_reqs); row_reqs
+// int32 ne = (N) or null; seq_lens int32 ne = (N); lse f32 ne = (n_heads, N) or
+// null; workspace: device memory of at least
+// cbx_paged_decode_attention_workspace(...) bytes.
+inline Tensor* paged_decode_attention(const Tensor& q, const Tensor& cache_k, const Tensor& cache_v,
+                                      const Tensor& block_table, const Tensor* row_reqs,
+                                      const Tensor& seq_lens, float scale, Tensor& out, Tensor* lse,
+                                      void* workspace, int64_t workspace_bytes, int32_t* err_word,
+                                      cbx_stream_t stream = nullptr) {
+    int64_t ps = 0;
+    const int64_t hd = q.ne[0], rows = q.ne[2];
+    if (!detail::paged_cache(cache_k, cache_v, &ps) || !detail::contiguous(q) ||
+        !detail::contiguous(out) || out.type != q.type || nelements(out) != nelements(q) ||
+        q.ne[3] != 1 || hd < 1 || cache_k.ne[0] % hd || nelements(seq_lens) != rows ||
+        (row_reqs && nelements(*row_reqs) != rows) || (lse && nelements(*lse) != q.ne[1] * rows)) {
+        std::fprintf(stderr, "paged_decode_attention: q, out and caches of matching sizes\n");
+        return nullptr;
+    }
+    return detail::report(
+        "paged_decode_attention",
+        cbx_paged_decode_attention(
+            q.data, q.type, 0, cache_k.data, cache_v.data, cache_k.type, cache_k.ne[2],
+            cache_k.ne[1], ps, static_cast<const int32_t*>(block_table.data), block_table.ne[1],
+            block_table.ne[0], row_reqs ? static_cast<const int32_t*>(row_reqs->data) : nullptr,
+            static_cast<const int32_t*>(seq_lens.data), rows, q.ne[1], cache_k.ne[0] / hd, hd, scale,
+            out.data, lse ? static_cast<float*>(lse->data) : nullptr, workspace, workspace_bytes,
+            err_word, stream),
+        &out);
+}
+
+// Log probabilities of given tokens under the rows of logits that the engine
+// reads back (t3.cpp:612-614): logits ne = (vocab, N) (uniform row stride);
+// tokens int32 ne = (N) and logprob f32 ne = (N), or both null; entropy f32 ne =
+// (N) or null; top_ids int32 and top_logprobs f32 ne = (top_k, N), or both null.
+inline Tensor* token_logprobs(const Tensor& logits, const Tensor* tokens, Tensor* logprob,
+                              Tensor* entropy, Tensor* top_ids, Tensor* top_logprobs,
+                              int32_t* err_word, cbx_stream_t stream = nullptr) {
+    int64_t sx = 0;
+    const int64_t n = nrows(logits);
+    if (!detail::uniform_rows(logits, &sx) || (tokens != nullptr) != (logprob != nullptr) ||
+        (tokens && (nelements(*tokens) != n || nelements(*logprob) != n)) ||
+        (entropy && nelements(*entropy) != n) || (top_ids != nullptr) != (top_logprobs != nullptr) ||
+        (top_ids && (nrows(*top_ids) != n || nelements(*top_logprobs) != nelements(*top_ids)))) {
+        std::fprintf(stderr, "token_logprobs: rows of logits and outputs of matching sizes\n");
+        return nullptr;
+    }
+    auto f32 = [](Tensor* t) { return t ? static_cast<float*>(t->data) : nullptr; };
+    return detail::report(
+        "token_logprobs",
+        cbx_token_logprobs(logits.data, logits.type, sx, n, logits.ne[0],
+                           tokens ? static_cast<const int32_t*>(tokens->data) : nullptr,
+                           top_ids ? top_ids->ne[0] : 0, f32(logprob), f32(entropy),
+                           top_ids ? static_cast<int32_t*>(top_ids->data) : nullptr,
+                           f32(top_logprobs), err_word, stream),
+        logprob ? logprob : entropy ? entropy : top_logprobs);
 }
 
 // The random inputs HiFTVocoder::generate_source draws when none are given
