@@ -18,8 +18,9 @@
 // Alternatives.  Each thread keeps the largest logit of every segment of its
 // elements.  The threads form 32 groups; the k-th largest of the 32 group
 // maxima, tau, is at most the k-th largest logit (k groups hold one at or above
-// it), so only segments whose largest reaches tau are read again, and their
-// elements at or above tau, a few dozen, are ranked by counting.  The order is
+// it), so only segments whose largest reaches tau are read again, by all
+// threads together, and their elements at or above tau, a few dozen, are ranked
+// by counting.  The order is
 // that of one 64-bit number per element (x as an ordered integer, then the
 // complement of its index), so ties fall to the lowest index and no two
 // elements are equal.  A row with more candidates than the list holds (a mask
@@ -212,6 +213,7 @@ struct Team {
     // where a team has little for each thread and latency counts.
     static constexpr int kUnroll = NT >= 256 ? 2 : 4;
     static constexpr int kCap = NT == 32 ? 128 : 512;   // candidates
+    static constexpr int kWork = NT == 32 ? 128 : 256;  // segments to read again
     static constexpr int kSegs = 16;                    // segments of a thread's elements
     struct Shared {
         float seg[kSegs * NT];
@@ -219,7 +221,8 @@ struct Team {
         float group[32];
         float s[kWarps], t[kWarps];
         unsigned long long key[kWarps];
-        int count;
+        int work[kWork];
+        int count, n_work;
     };
     static __device__ __forceinline__ void sync() {
         if constexpr (NT == 32) __syncwarp();
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
 
         // Maximum of the row, and of the 32 groups.
         float m = warp_max(top), group = top;
-        if (TOP && tid == 0) sh.count = 0;
+        if (TOP && tid == 0) sh.count = sh.n_work = 0;
         if constexpr (NT > 32) {
 #pragma unroll
             for (int o = 1; o < NT / 32; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
@@ -428,40 +431,45 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
         if constexpr (TOP) {
             float tau = m;
             if (a.top_k > 1) tau = __shfl_sync(0xffffffffu, sort_falling(group, lane), a.top_k - 1);
+            auto put = [&](int at, float v, int j) {
+                if (at < Tm::kCap) sh.list[at] = key_of(v, j);
+            };
             if (top >= tau && (tau != -INFINITY || row.V <= Tm::kCap)) {
-                auto put = [&](int at, float v, int j) {
-                    if (at < Tm::kCap) sh.list[at] = key_of(v, j);
-                };
                 if (tid < row.head && ends[0].x >= tau) put(atomicAdd(&sh.count, 1), ends[0].x, tid);
                 if (tid < row.V - row.tail && ends[0].y >= tau) put(atomicAdd(&sh.count, 1), ends[0].y, row.tail + tid);
                 uint32_t todo = 0;
                 for (int q = 0; q < n_segs; ++q) todo |= (sh.seg[q * NT + tid] >= tau ? 1u : 0u) << q;
-                for (; todo; todo &= todo - 1) {
-                    const int b0 = (__ffs(todo) - 1) * per;
-                    for (int b = b0; b < b0 + per && b < batches; ++b) {
-                        uint4 w[kUnroll];
-                        fetch(row, b, w);
-#pragma unroll
-                        for (int u = 0; u < kUnroll; ++u) {
-                            const uint4 one[1] = {w[u]};
-                            if (b * kBatch + u * NT + tid >= row.nv || max_of(one, T{}) < tau) continue;
-                            float2 f[EV / 2];
-                            widen<T, false>(w[u], f);
-                            int n = 0;
-#pragma unroll
-                            for (int e = 0; e < EV / 2; ++e) n += (f[e].x >= tau) + (f[e].y >= tau);
-                            if (!n) continue;  // all NaN
-                            int at = atomicAdd(&sh.count, n);
-                            const int j = row.first(b * kBatch + u * NT + tid);
-#pragma unroll
-                            for (int e = 0; e < EV / 2; ++e) {
-                                if (f[e].x >= tau) put(at++, f[e].x, j + 2 * e);
-                                if (f[e].y >= tau) put(at++, f[e].y, j + 2 * e + 1);
-                            }
-                        }
-                    }
+                if (todo) {
+                    int at = atomicAdd(&sh.n_work, __popc(todo));
+                    for (; todo && at < Tm::kWork; todo &= todo - 1, ++at)
+                        sh.work[at] = (__ffs(todo) - 1) * NT + tid;
                 }
             }
+            Tm::sync();
+            // The vectors of the listed segments, one for each thread: their owners
+            // alone would walk them one by one, their warps waiting.
+            const int n_work = sh.n_work, span = per * kUnroll;
+            if (n_work <= Tm::kWork)
+                for (int i = tid; i < n_work * span; i += NT) {
+                    const int item = i / span, of = sh.work[item];
+                    const int v = of % NT + (of / NT * span + (i - item * span)) * NT;
+                    if (v >= row.nv) continue;
+                    const uint4 w[1] = {row.vec(v)};
+                    if (max_of(w, T{}) < tau) continue;
+                    float2 f[EV / 2];
+                    widen<T, false>(w[0], f);
+                    int n = 0;
+#pragma unroll
+                    for (int e = 0; e < EV / 2; ++e) n += (f[e].x >= tau) + (f[e].y >= tau);
+                    if (!n) continue;  // all NaN
+                    int at = atomicAdd(&sh.count, n);
+                    const int j = row.first(v);
+#pragma unroll
+                    for (int e = 0; e < EV / 2; ++e) {
+                        if (f[e].x >= tau) put(at++, f[e].x, j + 2 * e);
+                        if (f[e].y >= tau) put(at++, f[e].y, j + 2 * e + 1);
+                    }
+                }
         }
         if (NT > 32 || TOP) Tm::sync();
         if constexpr (NT > 32) {
@@ -491,7 +499,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256
         }
         if constexpr (TOP) {
             const int n = sh.count;
-            if (!bad && n >= a.top_k && n <= Tm::kCap) {
+            if (!bad && sh.n_work <= Tm::kWork && n >= a.top_k && n <= Tm::kCap) {
                 for (int i = tid; i < n; i += NT) {
                     const unsigned long long key = sh.list[i];
                     int rank = 0;
