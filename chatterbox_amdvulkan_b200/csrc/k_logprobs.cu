@@ -312,7 +312,8 @@ __device__ __noinline__ void sums_from_differences(Row<T> row, int tid, float m,
 }
 
 template <typename T, int NT, bool TOP>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256 ? 5 : 1) k_token_logprobs(LogprobArgs a) {
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT <= 128 ? 7 : NT == 256 ? 5 : 1)
+k_token_logprobs(LogprobArgs a) {
     using Tm = Team<NT>;
     constexpr int EV = Vec<T>::n;
     constexpr int kTeams = NT < 128 ? 128 / NT : 1;  // rows at a time
@@ -536,16 +537,17 @@ int run_team(const LogprobArgs& a, cudaStream_t st) {
 }
 
 // Threads of a row.  A warp costs least per row, but needs many rows to fill
-// the GPU and is slow on a long one; a whole CTA is quickest on a single row.
-// Measured in us (B200; 32 / 128 / 256 / 512 threads a row):
-//   1 x 6563 f32          7.6 / 5.2 / 4.5 / 4.5
-//   1 x 50276 f32        38.7 / 12.0 / 9.9 / 7.2
-//   256 x 6563 f32       10.6 / 6.9 / 6.2 / 8.6
-//   1100 x 6563 f16      12.0 / 14.9 / 14.7 / 27.4
-//   1100 x 50276 f16     64.2 / 45.1 / 39.6 / 60.0
-//   2048 x 50276 f16    110.2 / 53.6 / 62.7 / 111.8
-//   4200 x 20000 bf16    66.8 / 57.5 / 61.6 / 131.4
-//   8192 x 6563 bf16     29.0 / 46.1 / 65.4 / 160.9
+// the GPU and is slow on a long one; a whole CTA is quickest on a single long
+// row.  Measured in us (B200; 32 / 128 / 256 / 512 threads a row):
+//   1 x 6563 f32, top 5          6.9 / 4.5 / 4.5 / 4.5
+//   1 x 50276 f32, top 5        29.8 / 10.3 / 9.3 / 7.6
+//   256 x 6563 f32, top 8        7.9 / 5.2 / 5.5 / 8.2
+//   1000 x 500 f16, top 8        5.2 / 6.5 / 13.7 / 67.3
+//   1100 x 6563 f16, top 8       8.2 / 12.4 / 13.7 / 28.7
+//   1100 x 50276 f16, top 8     41.8 / 40.9 / 37.3 / 61.6
+//   2048 x 50276 f16, top 20    67.6 / 45.5 / 57.5 / 110.4
+//   4200 x 20000 bf16, top 5    58.1 / 50.9 / 59.3 / 138.5
+//   8192 x 6563 bf16, top 1     27.7 / 42.7 / 68.4 / 170.6 (107.7 MB: 3.9 TB/s)
 // A row with less than a vector for each thread would leave groups without a
 // maximum and so without a bound for its alternatives: it takes fewer threads.
 // The warp's list holds the candidates of up to 24 alternatives (about 32 ln(1 /
@@ -555,8 +557,8 @@ int run_logprobs(const LogprobArgs& a, cudaStream_t st) {
     const int64_t rows = a.n_rows, sms = num_sms(), vecs = a.vocab / Vec<T>::n;
     const bool warp = a.top_k <= 24;
     if (warp && (vecs < 128 || (rows >= 7 * sms && vecs <= 2048))) return run_team<T, 32>(a, st);
-    if (rows <= sms && vecs >= 512) return run_team<T, 512>(a, st);
-    if (rows >= 10 * sms || vecs < 256) return run_team<T, 128>(a, st);
+    if (rows <= sms && vecs >= 2048) return run_team<T, 512>(a, st);
+    if (rows >= 10 * sms || vecs < 2048) return run_team<T, 128>(a, st);
     return run_team<T, 256>(a, st);
 }
 
