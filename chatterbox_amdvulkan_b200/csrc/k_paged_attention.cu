@@ -129,17 +129,23 @@ struct Work {
         lo = from < len ? (int)from : len;
         hi = to < len ? (int)to : len;
     }
-    // Cache row of a key; -1 behind the split's last and on a bad page.
-    __device__ __forceinline__ int find(const AttnArgs& a, int64_t key) {
+    // Block of a key, and its table entry (0 behind the split's last key).
+    __device__ __forceinline__ int block_of(const AttnArgs& a, int64_t key) const {
+        return a.page_shift >= 0 ? (int)key >> a.page_shift : (int)key / a.page_size;
+    }
+    __device__ __forceinline__ int entry(const AttnArgs& a, int64_t key) const {
+        return key < hi ? __ldg(table + block_of(a, key)) : 0;
+    }
+    // Cache row of a key, from its entry; -1 behind the split's last and on a bad page.
+    __device__ __forceinline__ int row_of(const AttnArgs& a, int page, int64_t key) {
         if (key >= hi) return -1;
-        const int blk = a.page_shift >= 0 ? (int)key >> a.page_shift : (int)key / a.page_size;
-        const int page = __ldg(table + blk);
         if (page < 0 || page >= a.n_pages) {
             flags |= CBX_EFLAG_PAGE_OOB;
             return -1;
         }
-        return page * a.page_rows + ((int)key - blk * a.page_size);
+        return page * a.page_rows + ((int)key - block_of(a, key) * a.page_size);
     }
+    __device__ __forceinline__ int find(const AttnArgs& a, int64_t key) { return row_of(a, entry(a, key), key); }
 };
 
 // Joins the states [W][G][state] of the CTA's warps (in shared memory, written
@@ -250,30 +256,6 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
     Work w(a, G, step);
     const int hi = w.hi;
 
-    // The query, scaled, this lane's elements.
-    float q[G][EL], acc[G][EL], m[G], l[G];
-    with_type(a.q, a.q_type, [&](auto* p) {
-        p += (int64_t)w.row * a.q_stride + (int64_t)w.head0 * hd;
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int v = 0; v < VPL; ++v)
-#pragma unroll
-                for (int e = 0; e < EV; ++e) {
-                    const int i = (v * VL + vl) * EV + e;
-                    q[g][v * EV + e] = g < w.heads && i < hd ? to_f(p[g * hd + i]) : 0.0f;
-                }
-    });
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < EL; ++e) {
-            q[g][e] *= a.scale_log2;
-            acc[g][e] = 0.0f;
-        }
-    }
     const char* kbase = static_cast<const char*>(a.ck) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
     const char* vbase = static_cast<const char*>(a.cv) + ((int64_t)w.kvh * hd + vl * EV) * sizeof(TC);
     const int64_t row_bytes = a.kv_dim * (int64_t)sizeof(TC);
@@ -310,14 +292,45 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
+    // The first table entries and the query are on their way together; with the
+    // ring, the first tiles too.
     int64_t t0 = w.lo + (int64_t)warp * TILE;
-    int slot = w.find(a, t0 + my_key), slot1 = -1, slot2 = -1, stage = 0;  // of this tile and the next two
+    const int entry0 = w.entry(a, t0 + my_key);
+    int slot = -1, slot1 = -1, slot2 = -1, stage = 0;  // cache rows of this tile and the next two
     if constexpr (RING) {
-        slot1 = w.find(a, t0 + step + my_key);
+        const int entry1 = w.entry(a, t0 + step + my_key), entry2 = w.entry(a, t0 + 2 * step + my_key);
+        slot = w.row_of(a, entry0, t0 + my_key);
+        slot1 = w.row_of(a, entry1, t0 + step + my_key);
+        slot2 = w.row_of(a, entry2, t0 + 2 * step + my_key);
         fetch(0, slot);
         fetch(1, slot1);
-        slot2 = w.find(a, t0 + 2 * step + my_key);
     }
+    // The query, scaled, this lane's elements.
+    float q[G][EL], acc[G][EL], m[G], l[G];
+    with_type(a.q, a.q_type, [&](auto* p) {
+        p += (int64_t)w.row * a.q_stride + (int64_t)w.head0 * hd;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+#pragma unroll
+                for (int e = 0; e < EV; ++e) {
+                    const int i = (v * VL + vl) * EV + e;
+                    q[g][v * EV + e] = g < w.heads && i < hd ? to_f(p[g * hd + i]) : 0.0f;
+                }
+    });
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EL; ++e) {
+            q[g][e] *= a.scale_log2;
+            acc[g][e] = 0.0f;
+        }
+    }
+    if constexpr (!RING) slot = w.row_of(a, entry0, t0 + my_key);
+
     for (; t0 < hi; t0 += step) {
         uint4 kr[U][VPL], vr[U][VPL];
         const bool there = slot >= 0;
@@ -538,6 +551,46 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
     grid_dep_launch();
     Work w(a, kMmaHeads, step);
 
+    float o[VECS][4] = {};
+    float m = -INFINITY, l = 0.0f;  // head g
+    const char* kbase = static_cast<const char*>(a.ck) + (int64_t)w.kvh * hd * 2;
+    const char* vbase = static_cast<const char*>(a.cv) + (int64_t)w.kvh * hd * 2;
+    const int64_t row_bytes = a.kv_dim * 2;
+    constexpr uint32_t kTileBytes = kMmaTile * HD * 2;
+    const uint32_t ring = smem_addr(smem) + warp * mma_ring_bytes<HD>();
+
+    // Puts the tile at t0 in a stage; returns which of its keys are there.
+    auto fetch = [&](int64_t t0, int stage, int slot) {
+        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
+        if (t0 < w.hi) {
+            constexpr int kRows = 32 / VECS;  // rows per instruction
+            const int r0 = lane / VECS, c = lane % VECS;
+            const uint32_t dst = ring + stage * 2 * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kMmaTile / kRows; ++i) {
+                const int r = i * kRows + r0;
+                const int s = __shfl_sync(0xffffffffu, slot, r);
+                const bool in = s >= 0 && c < vecs;
+                const int64_t off = in ? s * row_bytes + c * 16 : 0;
+                const uint32_t at = dst + r * (HD * 2) + ((c ^ (r & 7)) << 4);
+                copy16(at, kbase + off, in);
+                copy16(at + kTileBytes, vbase + off, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return there;
+    };
+
+    const int64_t first = w.lo + (int64_t)warp * kMmaTile;
+    uint64_t there = 0;  // 16 bits for each tile on its way, the oldest on top
+    int entries[kMmaStages], slot = -1;
+#pragma unroll
+    for (int s = 0; s < kMmaStages; ++s) entries[s] = w.entry(a, first + (int64_t)s * step + (lane & 15));
+#pragma unroll
+    for (int s = 0; s < kMmaStages; ++s) {
+        slot = w.row_of(a, entries[s], first + (int64_t)s * step + (lane & 15));
+        if (s < kMmaStages - 1) there = there << 16 | fetch(first + (int64_t)s * step, s, slot);
+    }
     // The first operand of S: head g.
     uint32_t qf[QT][KS][2];
     float scale = a.scale_log2;
@@ -580,44 +633,6 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < QT; ++k) qf[k][s][e] = f[k];
             }
-    }
-    float o[VECS][4] = {};
-    float m = -INFINITY, l = 0.0f;  // head g
-    const char* kbase = static_cast<const char*>(a.ck) + (int64_t)w.kvh * hd * 2;
-    const char* vbase = static_cast<const char*>(a.cv) + (int64_t)w.kvh * hd * 2;
-    const int64_t row_bytes = a.kv_dim * 2;
-    constexpr uint32_t kTileBytes = kMmaTile * HD * 2;
-    const uint32_t ring = smem_addr(smem) + warp * mma_ring_bytes<HD>();
-
-    // Puts the tile at t0 in a stage; returns which of its keys are there.
-    auto fetch = [&](int64_t t0, int stage, int slot) {
-        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
-        if (t0 < w.hi) {
-            constexpr int kRows = 32 / VECS;  // rows per instruction
-            const int r0 = lane / VECS, c = lane % VECS;
-            const uint32_t dst = ring + stage * 2 * kTileBytes;
-#pragma unroll
-            for (int i = 0; i < kMmaTile / kRows; ++i) {
-                const int r = i * kRows + r0;
-                const int s = __shfl_sync(0xffffffffu, slot, r);
-                const bool in = s >= 0 && c < vecs;
-                const int64_t off = in ? s * row_bytes + c * 16 : 0;
-                const uint32_t at = dst + r * (HD * 2) + ((c ^ (r & 7)) << 4);
-                copy16(at, kbase + off, in);
-                copy16(at + kTileBytes, vbase + off, in);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        return there;
-    };
-
-    const int64_t first = w.lo + (int64_t)warp * kMmaTile;
-    uint64_t there = 0;  // 16 bits for each tile on its way, the oldest on top
-    int slot = w.find(a, first + (lane & 15));
-#pragma unroll
-    for (int s = 0; s < kMmaStages - 1; ++s) {
-        there = there << 16 | fetch(first + s * step, s, slot);
-        slot = w.find(a, first + (int64_t)(s + 1) * step + (lane & 15));
     }
     int stage = 0;
     for (int64_t t0 = first; t0 < w.hi; t0 += step) {
@@ -713,14 +728,19 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
 }
 
 // Joins the splits' states of one row and head: first the weight of each split,
-// then the values, whose loads do not depend on one another.
-constexpr int kJoinThreads = 64;
+// then the values, 16 bytes a load, the splits shared by the threads so that a
+// thread's few loads travel together (one thread for all splits of an element
+// took 11 us for 36 splits, 32 us for 60).
+constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttnArgs a) {
     __shared__ float weight[kMaxSplits];
+    __shared__ float4 sums[kJoinThreads];
     grid_dep_wait();
     grid_dep_launch();
     const int64_t rh = blockIdx.x;
     const int sf = state_floats(a.head_dim), lane = threadIdx.x & 31;
+    const int vecs = a.head_dim / 4, parts = kJoinThreads / vecs;  // head_dim is 8 .. 256
+    const int v = threadIdx.x % vecs, part = threadIdx.x / vecs;
     const float* st = a.part + rh * a.splits * sf;
     // every warp for itself: kMaxSplits / 32 splits a lane
     float m[kMaxSplits / 32], l[kMaxSplits / 32], mm = -INFINITY, ll = 0.0f;
@@ -741,12 +761,28 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttnArgs a) {
     }
     ll = warp_sum(ll);
     __syncthreads();
-    const float r = ll != 0.0f ? 1.0f / ll : 0.0f;
-    for (int e = threadIdx.x; e < a.head_dim; e += kJoinThreads) {
-        float o = 0.0f;
-#pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) o = fmaf(weight[s], st[s * sf + kStateHead + e], o);
-        store_elem(a.out, a.q_type, rh * a.head_dim + e, o * r);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (part < parts) {
+#pragma unroll 4
+        for (int s = part; s < a.splits; s += parts) {
+            const float4 x = *reinterpret_cast<const float4*>(st + s * sf + kStateHead + 4 * v);
+            const float c = weight[s];
+            o = make_float4(fmaf(c, x.x, o.x), fmaf(c, x.y, o.y), fmaf(c, x.z, o.z), fmaf(c, x.w, o.w));
+        }
+        sums[threadIdx.x] = o;
+    }
+    __syncthreads();
+    if (part == 0) {
+        for (int p = 1; p < parts; ++p) {
+            const float4 x = sums[p * vecs + v];
+            o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+        }
+        const float r = ll != 0.0f ? 1.0f / ll : 0.0f;
+        const int64_t at = rh * a.head_dim + 4 * v;
+        store_elem(a.out, a.q_type, at, o.x * r);
+        store_elem(a.out, a.q_type, at + 1, o.y * r);
+        store_elem(a.out, a.q_type, at + 2, o.z * r);
+        store_elem(a.out, a.q_type, at + 3, o.w * r);
     }
     if (a.lse && threadIdx.x == 0) a.lse[rh] = lse_of(mm, ll);
 }
@@ -785,7 +821,7 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
     for (int64_t n = 1; n <= (max_keys >= 8192 ? kMaxSplits : kMaxCluster) && n <= steps; ++n) {
         const int64_t waves = (ctas * n + resident - 1) / resident;
         const int64_t cost = waves * ((steps + n - 1) / n * step + 512) +
-                             (n == 1 ? 0 : n <= kMaxCluster ? 256 : 512 + 24 * n);
+                             (n == 1 ? 0 : n <= kMaxCluster ? 256 : 320 + 16 * n);
         if (n == 1 || cost < least) {
             least = cost;
             best = n;
