@@ -5,7 +5,11 @@
 //
 // A copy with a scattered destination, bound by HBM: the GEMM's row is read
 // once and its parts are written once.  A thread keeps one column group of 8
-// elements (its bias stays in registers) and walks rows.
+// elements (its bias stays in registers) and walks rows; rows narrower than the
+// CTA lie side by side in it.  Measured (B200): 65,536 rows of 1024 + 2 x 1024
+// f32 into bf16 pages 193 us (1.34 GB, 6.9 TB/s: above the copy rate, as part of
+// what is written stays in L2); 54,170 rows of 256 + 2 x 64 f16 14.7 us (83 MB,
+// 5.7 TB/s; 21.5 us with one row abreast); one row 1.5 us.
 #include "cbx_common.cuh"
 
 namespace cbx {
@@ -27,6 +31,7 @@ struct PagedAppendArgs {
     int page_size;
     int n_slots;
     bool dense;  // page_stride == page_size * kd: a slot is a row of the cache
+    int cols;  // column groups of a CTA (vector kernel)
     void* q;
     int32_t* err;
 };
@@ -37,14 +42,26 @@ __device__ __forceinline__ int64_t slot_offset(const PagedAppendArgs& a, int slo
     return (int64_t)page * a.page_stride + (int64_t)(slot - page * a.page_size) * a.kd;
 }
 
+// Rows in flight per thread, waiting in registers as they are in memory: 4 of 16
+// bits, 2 of f32.  52,428 rows of 1280 + 2 x 320 bf16, in us, 1 / 2 / 3 / 4 rows:
+// 132 / 74 / 65 / 63; the f32 rows above 270 / 193 / 195 / 195.  Widened on
+// arrival, 4 rows took 72 registers, and the bf16 ones 99 us.
+template <typename TI>
+constexpr int rows_in_flight() {
+    return sizeof(TI) == 2 ? 4 : 2;
+}
+
 // qd, kd, row strides multiples of 8; all rows 16-byte aligned.
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kThreads) k_paged_append_vec(PagedAppendArgs a) {
-    constexpr int kRows = 4;  // rows in flight per thread
+    constexpr int kRows = rows_in_flight<TI>();
+    constexpr int kVecs = kCols * sizeof(TI) / 16;
     grid_dep_wait();
     grid_dep_launch();
-    const int g = blockIdx.x * kThreads + threadIdx.x;
-    if (g >= (a.qd + 2 * a.kd) / kCols) return;
+    const int side = threadIdx.x / a.cols;  // of the rows side by side
+    const int abreast = kThreads / a.cols;
+    const int g = blockIdx.x * a.cols + threadIdx.x % a.cols;
+    if (side >= abreast || g >= (a.qd + 2 * a.kd) / kCols) return;
     const int col = g * kCols;
     const int part = col < a.qd ? 0 : col < a.qd + a.kd ? 1 : 2;
     const int in_part = part == 0 ? col : part == 1 ? col - a.qd : col - a.qd - a.kd;
@@ -52,28 +69,40 @@ __global__ void __launch_bounds__(kThreads) k_paged_append_vec(PagedAppendArgs a
     float b[kCols] = {};
     if (a.bias) ldv<float, kCols>(a.bias + col, b);
     const TI* src = static_cast<const TI*>(a.qkv) + col;
-    for (int64_t r0 = (int64_t)blockIdx.y * kRows; r0 < a.n_rows; r0 += (int64_t)gridDim.y * kRows) {
-        float x[kRows][kCols];
+    const int64_t stride = (int64_t)gridDim.y * abreast * kRows;
+    for (int64_t r0 = ((int64_t)blockIdx.y * abreast + side) * kRows; r0 < a.n_rows; r0 += stride) {
+        uint4 raw[kRows][kVecs];
         int slot[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             slot[i] = -1;
             if (r0 + i < a.n_rows) {
                 slot[i] = __ldg(a.slots + r0 + i);
-                ldv<TI, kCols>(src + (r0 + i) * a.qkv_stride, x[i]);
+#pragma unroll
+                for (int v = 0; v < kVecs; ++v)
+                    raw[i][v] = __ldg(reinterpret_cast<const uint4*>(src + (r0 + i) * a.qkv_stride) + v);
             }
         }
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             if (slot[i] == -1) continue;
+            float x[kCols];
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) x[i][j] = __fadd_rn(x[i][j], b[j]);
+            for (int v = 0; v < kVecs; ++v) {
+                constexpr int k = 4 / (int)sizeof(TI);
+                unpack32(raw[i][v].x, x + (4 * v) * k, TI{});
+                unpack32(raw[i][v].y, x + (4 * v + 1) * k, TI{});
+                unpack32(raw[i][v].z, x + (4 * v + 2) * k, TI{});
+                unpack32(raw[i][v].w, x + (4 * v + 3) * k, TI{});
+            }
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) x[j] = __fadd_rn(x[j], b[j]);
             const bool good = slot[i] >= 0 && slot[i] < a.n_slots;
             if (!good && col == 0) atomicOr(a.err, CBX_EFLAG_PAGE_OOB);
             if (part == 0) {
-                if (a.q) stv<TI, kCols>(static_cast<TI*>(a.q) + (r0 + i) * a.qd + in_part, x[i]);
+                if (a.q) stv<TI, kCols>(static_cast<TI*>(a.q) + (r0 + i) * a.qd + in_part, x);
             } else if (good) {
-                stv<TC, kCols>(cache + slot_offset(a, slot[i]) + in_part, x[i]);
+                stv<TC, kCols>(cache + slot_offset(a, slot[i]) + in_part, x);
             }
         }
     }
@@ -106,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_append_scalar(PagedAppendArg
 }
 
 template <typename TI, typename TC>
-int run_append(const PagedAppendArgs& a, cudaStream_t st) {
+int run_append(PagedAppendArgs a, cudaStream_t st) {
     auto rows16 = [](const void* p, int64_t stride, size_t size) {
         return aligned16(p) && (stride * (int64_t)size) % 16 == 0;
     };
@@ -115,8 +144,10 @@ int run_append(const PagedAppendArgs& a, cudaStream_t st) {
                      (!a.q || aligned16(a.q)) && rows16(a.ck, a.page_stride, sizeof(TC)) &&
                      rows16(a.cv, a.page_stride, sizeof(TC));
     const int64_t units = vec ? (a.qd + 2LL * a.kd) / kCols : a.qd + 2LL * a.kd;
-    const unsigned gx = (unsigned)((units + kThreads - 1) / kThreads);
-    const int64_t want = vec ? (a.n_rows + 3) / 4 : a.n_rows;
+    a.cols = vec && units < kThreads ? (int)units : kThreads;
+    const unsigned gx = (unsigned)((units + a.cols - 1) / a.cols);
+    const int64_t per_cta = vec ? rows_in_flight<TI>() * (kThreads / a.cols) : 1;
+    const int64_t want = (a.n_rows + per_cta - 1) / per_cta;
     const unsigned gy = (unsigned)(want < 65535 ? want : 65535);
     cudaError_t e = vec ? launch(k_paged_append_vec<TI, TC>, dim3(gx, gy), dim3(kThreads), 0, st, a)
                         : launch(k_paged_append_scalar<TI, TC>, dim3(gx, gy), dim3(kThreads), 0, st, a);
@@ -167,7 +198,7 @@ extern "C" CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type,
         return fail(CBX_ERR_INVALID_ARG, "%s: NULL qkv, slots, cache or err_word", name);
     PagedAppendArgs a{qkv, qkv_row_stride, qkv_bias, n_rows, (int)q_dim, (int)kv_dim, slots,
                       cache_k, cache_v, page_stride, (int)page_size, (int)(n_pages * page_size),
-                      page_stride == page_size * kv_dim, q_out, err_word};
+                      page_stride == page_size * kv_dim, 0, q_out, err_word};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (qkv_type) {
         case CBX_TYPE_F32: return run_cache<float>(a, cache_type, st);

@@ -535,9 +535,10 @@ __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tile
 // bytes a lane, consecutive lanes on consecutive bytes of a key's row), so no
 // CTA barrier stands in the loop, and two tiles are on their way while one is
 // worked on.  Loading the operands' layouts straight from global memory moved
-// the same bytes in 4 times the requests (quarter lines of V): 122 us against
-// 57 us for one row of 65,537 keys, 32 heads over 8 of 128 in bf16 (4.7 TB/s);
-// f32 FMAs with 4 heads a CTA take 107 us there.  The 16-byte vectors of a row are permuted by the
+// the same bytes in 4 times the requests (quarter lines of V): 122 us for one
+// row of 65,537 keys, 32 heads over 8 of 128 in bf16, against 57 us with the
+// ring (both with the first form of the join; 50 us, 5.4 TB/s, now).  f32 FMAs
+// with 4 heads a CTA took 107 us there.  The 16-byte vectors of a row are permuted by the
 // row's number, which keeps ldmatrix free of bank conflicts.
 template <typename T, int HD, int QT, int PT>
 __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
@@ -803,10 +804,10 @@ struct Splits {
 // joining in a cluster costs little, over the workspace a second launch.
 // Measured in us (B200), splits 1 / 4 / 8 in a cluster, 16 / 32 / 48 over the
 // workspace:
-//   1 row, 1000 keys, 16 kv heads of 64, f32     9.6 / 5.5 / 5.0, 10.0 / 14.7 / 23.4
-//   1 row, 65,537 keys, 8 kv heads of 128, bf16  708 / - / 98, 60 / 57 / 77
-//   64 rows up to 2048, 16 kv heads of 64, f16   56 / 105 / 182
-// (Clusters of 16 were no faster than 16 splits over the workspace: 65 us.)
+//   1 row, 1000 keys, 16 kv heads of 64, f32     9.7 / 5.5 / 5.2, 7.0 / 10.1 / 12.0
+//   1 row, 65,537 keys, 8 kv heads of 128, bf16  711 / 187 / 97, 55 / 48 / 62
+//   64 rows up to 2048, 16 kv heads of 64, f16   56 / 101 / 175
+// (A cluster of 16 took 65 us for the second.)
 Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, int cache_type,
                      int64_t max_keys) {
     const bool mma = use_mma(cache_type, group, (int)head_dim);
@@ -854,7 +855,7 @@ cudaError_t run_fma_heads(AttnArgs a, int64_t n_rows, cudaStream_t st) {
 // Four query heads take the ring, one and two the registers, in us (B200):
 //   94 rows of 2511 keys, 16 heads over 2 of 64, f32       113 / 169
 //   7 rows of 1922 keys, 32 heads over 16 of 128, f32       46 / 40
-//   128 rows up to 8196 keys, 16 heads of 64, bf16         340 / 312
+//   128 rows up to 8196 keys, 16 heads of 64, bf16         340 / 312 (1.98 GB: 6.3 TB/s)
 template <typename TC, int VL, int VPL>
 cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
     switch (group_chunk(a.group)) {
