@@ -3,7 +3,8 @@
  * fused per-layer elementwise ops that the Chatterbox TTS engine runs between
  * its GEMMs (T3 embedding gather-add, residual-add + LayerNorm, GELU-tanh,
  * SiLU, Mish, channel-strided LayerNorm + Mish for the CFM estimator, the
- * sinusoidal timestep embedding and HiFT's Snake).
+ * sinusoidal timestep embedding and HiFT's Snake), their neighbours, and a
+ * decode step's operators on a paged KV cache.
  *
  * Each entry point replaces one layer helper of chatterbox-cpp (or the chain
  * of ggml graph nodes it emits); the citation above each declaration names the
