@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
 #pragma unroll
                 for (int e = 0; e < EL; ++e) acc[g][e] *= c;
             }
-            p[g] = there ? ex2_approx(s - m[g]) : 0.0f;
+            p[g] = s == -INFINITY ? 0.0f : ex2_approx(s - m[g]);  // whatever m is: it may be -inf too
             l[g] += p[g];
         }
 #pragma unroll
@@ -670,11 +670,10 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
             }
         }
         float best = m;
-        bool in[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            in[i] = keys >> (2 * t + (i & 1) + (i >> 1) * 8) & 1;
-            s[i] = in[i] ? s[i] * scale : -INFINITY;
+            const bool in = keys >> (2 * t + (i & 1) + (i >> 1) * 8) & 1;
+            s[i] = in ? s[i] * scale : -INFINITY;
             best = fmaxf(best, s[i]);
         }
         if (__any_sync(0xffffffffu, best > m)) {
@@ -691,8 +690,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
         uint32_t pf[2][PT];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float p0 = in[2 * n] ? ex2_approx(s[2 * n] - m) : 0.0f;
-            const float p1 = in[2 * n + 1] ? ex2_approx(s[2 * n + 1] - m) : 0.0f;
+            const float p0 = s[2 * n] == -INFINITY ? 0.0f : ex2_approx(s[2 * n] - m);
+            const float p1 = s[2 * n + 1] == -INFINITY ? 0.0f : ex2_approx(s[2 * n + 1] - m);
             l += p0 + p1;
             terms_of<T, PT>(p0, p1, pf[n]);
         }

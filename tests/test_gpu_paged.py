@@ -305,6 +305,24 @@ def test_attention_infinities_and_nan_of_real_keys(ops):
     assert out[3, 0, 5] == math.inf and out[3, 0, :5].isfinite().all()
 
 
+@pytest.mark.parametrize("qt,ct,H,Hk", [(F32, F32, 2, 1), (F16, F16, 8, 2), (BF16, BF16, 2, 2), (F32, F32, 8, 1)])
+def test_attention_scores_of_minus_infinity(ops, qt, ct, H, Hk):
+    """Whole tiles of keys whose score is -inf weigh nothing; where all are, the row counts as empty."""
+    q, ck, cv, table, n = make([700, 700, 90], H, Hk, 64, 16, qt, ct, 11)
+    q.abs_().clamp_(min=0.01)
+    gone = torch.zeros(700, dtype=torch.bool)
+    gone[:300], gone[310:690] = True, True
+    for b, mask in ((0, gone), (2, torch.ones(90, dtype=torch.bool))):
+        at = torch.arange(len(mask), device="cuda")[mask.cuda()]
+        ck[table[b].long()[at // 16], at % 16] = -math.inf
+    out, lse = ops.paged_decode_attention(q, ck, cv, table, n, return_lse=True)
+    left = torch.arange(700, device="cuda")[~gone.cuda()]
+    k, v = (c[table[0].long()[left // 16], left % 16][None].contiguous() for c in (ck, cv))
+    check_attention(out[:1], attention_ref(q[:1], k, v, ints([[0]]), ints([len(left)])), lse[:1])
+    check_attention(out[1:2], attention_ref(q[1:2], ck, cv, table[1:2], n[1:2]), lse[1:2])
+    assert not out[2].any() and (lse[2] == -math.inf).all()
+
+
 def test_attention_many_rows_of_one_request(ops):
     """row_reqs: the tokens of a prefill chunk, each row with its own length, and unordered requests."""
     q, ck, cv, table, n = make([50, 20, 33], 4, 2, 64, 16, F32, F16, 7)
