@@ -98,15 +98,19 @@ constexpr int kStateHead = 4;  // floats before acc: m, l, two unused
 __host__ __device__ inline int state_floats(int head_dim) { return kStateHead + head_dim; }
 
 // What a CTA works on: a row, one kv head with up to G of its query heads, and
-// one split's keys [lo, hi), whole steps of the CTA.
+// one split's keys [lo, hi), whole steps of the CTA.  Splits lie side by side in
+// the grid (a cluster), then the heads of a row, which read the same lines.
 struct Work {
-    int row, kvh, head0, heads, lo, hi;
+    int row, split, kvh, head0, heads, lo, hi;
     const int32_t* table;
     int flags;
     __device__ __forceinline__ Work(const AttnArgs& a, int chunk_heads, int step) {
-        row = blockIdx.z;
-        kvh = blockIdx.y / a.chunks;
-        const int first = blockIdx.y % a.chunks * chunk_heads;
+        const int cta = blockIdx.x / a.splits, per_row = a.n_kv * a.chunks;
+        split = blockIdx.x - cta * a.splits;
+        row = cta / per_row;
+        const int hc = cta - row * per_row;
+        kvh = hc / a.chunks;
+        const int first = (hc - kvh * a.chunks) * chunk_heads;
         head0 = kvh * a.group + first;
         heads = a.group - first < chunk_heads ? a.group - first : chunk_heads;
         flags = 0;
@@ -124,8 +128,8 @@ struct Work {
         }
         table = a.table + (int64_t)req * a.max_blocks;
         const int64_t steps = ((int64_t)len + step - 1) / step;
-        const int64_t from = steps * blockIdx.x / a.splits * step;
-        const int64_t to = steps * (blockIdx.x + 1) / a.splits * step;
+        const int64_t from = steps * split / a.splits * step;
+        const int64_t to = steps * (split + 1) / a.splits * step;
         lo = from < len ? (int)from : len;
         hi = to < len ? (int)to : len;
     }
@@ -170,7 +174,7 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Work& w, float* 
         }
         const int64_t rh = (int64_t)w.row * a.n_heads + w.head0 + g;
         if (a.splits > 1) {
-            float* st = a.cluster ? own + g * sf : a.part + (rh * a.splits + blockIdx.x) * sf;
+            float* st = a.cluster ? own + g * sf : a.part + (rh * a.splits + w.split) * sf;
             if (e == 0) {
                 st[0] = mm;
                 st[1] = ll;
@@ -184,7 +188,7 @@ __device__ __forceinline__ void finish(const AttnArgs& a, const Work& w, float* 
     if (!a.cluster) return;
     cluster_sync();
     // Each CTA of the cluster joins its share of the values.
-    for (int i = blockIdx.x * (W * 32) + threadIdx.x; i < w.heads * hd; i += a.splits * (W * 32)) {
+    for (int i = w.split * (W * 32) + threadIdx.x; i < w.heads * hd; i += a.splits * (W * 32)) {
         const int g = i / hd, e = i % hd;
         const uint32_t st = smem_addr(own + g * sf);
         float m[kMaxCluster], l[kMaxCluster], v[kMaxCluster];
@@ -816,6 +820,7 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
                        : 8 * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
     const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? 4 : 2);
     const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
+    if (ctas >= 8 * resident) return {1, false};
     const int64_t steps = (max_keys + step - 1) / step;
     int64_t least = 0, best = 1;
     for (int64_t n = 1; n <= (max_keys >= 8192 ? kMaxSplits : kMaxCluster) && n <= steps; ++n) {
@@ -832,7 +837,7 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
 
 cudaError_t launch_attend(void (*kern)(AttnArgs), int warps, size_t smem, const AttnArgs& a,
                           int64_t n_rows, cudaStream_t st) {
-    const dim3 grid((unsigned)a.splits, (unsigned)(a.n_kv * a.chunks), (unsigned)n_rows);
+    const dim3 grid((unsigned)(n_rows * a.n_kv * a.chunks * a.splits));  // below 2^31: n_rows * n_heads is
     if (a.cluster) return launch_cluster(kern, grid, dim3(warps * 32), smem, (unsigned)a.splits, st, a);
     cudaError_t e = launch(kern, grid, dim3(warps * 32), smem, st, a);
     if (e == cudaSuccess && a.splits > 1)
@@ -896,11 +901,13 @@ cudaError_t run_head(const AttnArgs& a, int cache_type, int64_t n_rows, cudaStre
 int check_sizes(const char* name, int64_t n_rows, int64_t n_heads, int64_t n_kv_heads,
                 int64_t head_dim, int64_t max_blocks, int64_t page_size, int cache_type) {
     constexpr int64_t kInt = 2147483647;
-    if (n_rows < 0 || n_rows > 65535)
-        return fail(CBX_ERR_INVALID_ARG, "%s: n_rows %lld outside [0, 65535]", name, (long long)n_rows);
+    if (n_rows < 0 || n_rows > kInt)
+        return fail(CBX_ERR_INVALID_ARG, "%s: n_rows %lld", name, (long long)n_rows);
     if (n_kv_heads <= 0 || n_heads <= 0 || n_heads > 65535 || n_heads % n_kv_heads)
         return fail(CBX_ERR_INVALID_ARG, "%s: n_heads %lld is not a multiple of n_kv_heads %lld",
                     name, (long long)n_heads, (long long)n_kv_heads);
+    if (n_rows > kInt / n_heads)
+        return fail(CBX_ERR_INVALID_ARG, "%s: n_rows * n_heads is 2^31 or more", name);
     if (head_dim < 8 || head_dim > 256 || head_dim % 8)
         return fail(CBX_ERR_INVALID_ARG, "%s: head_dim %lld is not a multiple of 8 up to 256", name,
                     (long long)head_dim);

@@ -504,7 +504,7 @@ CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_r
  * sums and raise CBX_EFLAG_PAGE_OOB, a row_reqs entry outside [0, n_reqs) does
  * too (the row counts as empty); a length above max_blocks * page_size or below
  * 0 is clamped and raises CBX_EFLAG_LENGTH.
- * n_rows <= 65535; head_dim: a multiple of 8, at most 256; caches 16-byte aligned, page_stride a
+ * n_rows * n_heads below 2^31; head_dim: a multiple of 8, at most 256; caches 16-byte aligned, page_stride a
  * multiple of kv_dim and the cache at most 2^31 - 1 rows of kv_dim long
  * (n_pages * page_stride / kv_dim).  out and lse must not overlap the inputs.
  * workspace: device memory of cbx_paged_decode_attention_workspace(...) bytes,

@@ -333,6 +333,17 @@ def test_attention_many_rows_of_one_request(ops):
     check_attention(out, attention_ref(q, ck, cv, table, ints(lens), ints(reqs)), lse)
 
 
+def test_attention_of_more_rows_than_a_grid_dimension_holds(ops):
+    """The rows of a large prefill: 70,000, most of them equal, checked against a few."""
+    q, ck, cv, table, n = make([9, 4], 4, 2, 32, 4, F32, F16, 12)
+    N = 70000
+    r = torch.arange(N, device="cuda")
+    reqs, lens = (r % 2).to(torch.int32), (1 + r % 4).to(torch.int32)
+    out = ops.paged_decode_attention(q[r % 2].contiguous(), ck, cv, table, lens, row_reqs=reqs)
+    check_attention(out[:4], attention_ref(q[r[:4] % 2], ck, cv, table, lens[:4], reqs[:4]))
+    assert torch.equal(out, out[:4].repeat(N // 4, 1, 1))
+
+
 def test_attention_bad_indexes_are_left_out(ops):
     q, ck, cv, table, n = make([40, 40, 40, 40], 2, 1, 64, 8, F32, F32, 8)
     bad = table.clone()

@@ -78,7 +78,7 @@ def attn_args(**kw):
 
 
 @pytest.mark.parametrize("kw,status,msg", [
-    (dict(rows=-1), -1, "n_rows"), (dict(rows=65536), -1, "n_rows"), (dict(H=5), -1, "multiple"),
+    (dict(rows=-1), -1, "n_rows"), (dict(rows=1 << 31), -1, "n_rows"), (dict(rows=1 << 29, reqs=1 << 29), -1, "2^31"), (dict(H=5), -1, "multiple"),
     (dict(Hk=0), -1, "multiple"), (dict(hd=60), -1, "head_dim"), (dict(hd=264), -1, "head_dim"),
     (dict(hd=0), -1, "head_dim"), (dict(mb=0), -1, "max_blocks"), (dict(page=0), -1, "page_size"),
     (dict(pages=0), -1, "n_pages"), (dict(ps=16 * 128 - 128), -1, "page_stride"),
