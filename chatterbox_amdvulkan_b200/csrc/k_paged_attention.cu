@@ -810,6 +810,8 @@ struct Splits {
 //   1 row, 1000 keys, 16 kv heads of 64, f32     9.7 / 5.5 / 5.2, 7.0 / 10.1 / 12.0
 //   1 row, 65,537 keys, 8 kv heads of 128, bf16  711 / 187 / 97, 55 / 48 / 62
 //   64 rows up to 2048, 16 kv heads of 64, f16   56 / 101 / 175
+//   27 rows, 577 keys, 16 heads over 4 of 64, f32 q, bf16   splits 1 2 3 4: 11.3 9.6 9.4 14.0
+//   5 rows, 7035 keys, 16 heads of 64, bf16                 splits 1 2 3 4: 49 36 29 39
 // (A cluster of 16 took 65 us for the second.)
 Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, int cache_type,
                      int64_t max_keys) {
@@ -818,13 +820,17 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
     const int64_t vecs = head_dim * type_size(cache_type) / 16;
     const int64_t step = mma ? kMmaTile * kMmaWarps
                        : 8 * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
-    const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? 4 : 2);
+    // CTAs per SM by registers (and shared memory): the tensor-core kernel's f32
+    // queries take 3 terms, and so more registers, on bf16 caches only.
+    const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? (cache_type == CBX_TYPE_F16 ? 4 : 3) : 2);
     const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
     if (ctas >= 8 * resident) return {1, false};
     const int64_t steps = (max_keys + step - 1) / step;
     int64_t least = 0, best = 1;
     for (int64_t n = 1; n <= (max_keys >= 8192 ? kMaxSplits : kMaxCluster) && n <= steps; ++n) {
-        const int64_t waves = (ctas * n + resident - 1) / resident;
+        // a cluster must fit into one GPC: not quite all places can be taken
+        const int64_t places = n > 1 && n <= kMaxCluster ? resident * 97 / 100 : resident;
+        const int64_t waves = (ctas * n + places - 1) / places;
         const int64_t cost = waves * ((steps + n - 1) / n * step + 512) +
                              (n == 1 ? 0 : n <= kMaxCluster ? 256 : 320 + 16 * n);
         if (n == 1 || cost < least) {
