@@ -229,6 +229,19 @@ __device__ __forceinline__ uint4 lds16(uint32_t p) {
     return v;
 }
 
+// The elements of a 16-byte vector as pairs of f32, for the packed FMAs.
+template <typename TC, int N>
+__device__ __forceinline__ void pairs_of(uint4 w, float2 (&f)[N], TC) {
+    constexpr int k = 4 / (int)sizeof(TC);
+    float g[2 * N];
+    unpack32(w.x, g, TC{});
+    unpack32(w.y, g + k, TC{});
+    unpack32(w.z, g + 2 * k, TC{});
+    unpack32(w.w, g + 3 * k, TC{});
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
+}
+
 // Shape of the FMA kernel.  With one or two query heads, a tile of keys and one
 // of values wait in registers (8 loads each).  With more, the registers belong
 // to the heads, so the loads go through a ring in shared memory, two tiles
@@ -310,7 +323,8 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
         fetch(1, slot1);
     }
     // The query, scaled, this lane's elements.
-    float q[G][EL], acc[G][EL], m[G], l[G];
+    float2 q[G][EL / 2], acc[G][EL / 2];
+    float m[G], l[G];
     with_type(a.q, a.q_type, [&](auto* p) {
         p += (int64_t)w.row * a.q_stride + (int64_t)w.head0 * hd;
 #pragma unroll
@@ -318,9 +332,10 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
 #pragma unroll
             for (int v = 0; v < VPL; ++v)
 #pragma unroll
-                for (int e = 0; e < EV; ++e) {
-                    const int i = (v * VL + vl) * EV + e;
-                    q[g][v * EV + e] = g < w.heads && i < hd ? to_f(p[g * hd + i]) : 0.0f;
+                for (int e = 0; e < EV; e += 2) {
+                    const int i = (v * VL + vl) * EV + e;  // head_dim is even: both or neither
+                    const bool in = g < w.heads && i < hd;
+                    q[g][(v * EV + e) / 2] = make_float2(in ? to_f(p[g * hd + i]) : 0.0f, in ? to_f(p[g * hd + i + 1]) : 0.0f);
                 }
     });
 #pragma unroll
@@ -328,9 +343,9 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
         m[g] = -INFINITY;
         l[g] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < EL; ++e) {
-            q[g][e] *= a.scale_log2;
-            acc[g][e] = 0.0f;
+        for (int e = 0; e < EL / 2; ++e) {
+            q[g][e] = __fmul2_rn(q[g][e], pair(a.scale_log2));
+            acc[g][e] = pair(0.0f);
         }
     }
     if constexpr (!RING) slot = w.row_of(a, entry0, t0 + my_key);
@@ -374,18 +389,15 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
             float d[U];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                d[j] = 0.0f;
+                float2 sum = pair(0.0f);
 #pragma unroll
                 for (int v = 0; v < VPL; ++v) {
-                    constexpr int kPer32 = 4 / (int)sizeof(TC);
-                    float f[EV];
-                    unpack32(kr[j][v].x, f, TC{});
-                    unpack32(kr[j][v].y, f + kPer32, TC{});
-                    unpack32(kr[j][v].z, f + 2 * kPer32, TC{});
-                    unpack32(kr[j][v].w, f + 3 * kPer32, TC{});
+                    float2 f[EV / 2];
+                    pairs_of(kr[j][v], f, TC{});
 #pragma unroll
-                    for (int e = 0; e < EV; ++e) d[j] = fmaf(q[g][v * EV + e], f[e], d[j]);
+                    for (int e = 0; e < EV / 2; ++e) sum = __ffma2_rn(q[g][v * EV / 2 + e], f[e], sum);
                 }
+                d[j] = sum.x + sum.y;
             }
             // Sum each d[j] over the VL lanes of its key: the lanes exchange
             // halves of the values until one is left, then add up.
@@ -411,22 +423,18 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
                 m[g] = t;
                 l[g] *= c;
 #pragma unroll
-                for (int e = 0; e < EL; ++e) acc[g][e] *= c;
+                for (int e = 0; e < EL / 2; ++e) acc[g][e] = __fmul2_rn(acc[g][e], pair(c));
             }
             p[g] = s == -INFINITY ? 0.0f : ex2_approx(s - m[g]);  // whatever m is: it may be -inf too
             l[g] += p[g];
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            float f[VPL][EV];
+            float2 f[VPL][EV / 2];
 #pragma unroll
             for (int v = 0; v < VPL; ++v) {
-                constexpr int kPer32 = 4 / (int)sizeof(TC);
                 if constexpr (RING) vr[j][v] = landed(1, j, v);
-                unpack32(vr[j][v].x, f[v], TC{});
-                unpack32(vr[j][v].y, f[v] + kPer32, TC{});
-                unpack32(vr[j][v].z, f[v] + 2 * kPer32, TC{});
-                unpack32(vr[j][v].w, f[v] + 3 * kPer32, TC{});
+                pairs_of(vr[j][v], f[v], TC{});
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -434,7 +442,8 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
 #pragma unroll
                 for (int v = 0; v < VPL; ++v)
 #pragma unroll
-                    for (int e = 0; e < EV; ++e) acc[g][v * EV + e] = fmaf(w, f[v][e], acc[g][v * EV + e]);
+                    for (int e = 0; e < EV / 2; ++e)
+                        acc[g][v * EV / 2 + e] = __ffma2_rn(pair(w), f[v][e], acc[g][v * EV / 2 + e]);
             }
         }
         if (RING) stage = stage == 2 ? 0 : stage + 1;
@@ -455,9 +464,12 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
         for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         l[g] = t;
 #pragma unroll
-        for (int e = 0; e < EL; ++e)
+        for (int e = 0; e < EL / 2; ++e)
 #pragma unroll
-            for (int o = VL; o < 32; o <<= 1) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
+            for (int o = VL; o < 32; o <<= 1) {
+                acc[g][e].x += __shfl_xor_sync(0xffffffffu, acc[g][e].x, o);
+                acc[g][e].y += __shfl_xor_sync(0xffffffffu, acc[g][e].y, o);
+            }
         float* st = states + (warp * G + g) * sf;
         if (lane == 0) {
             st[0] = m[g];
@@ -469,7 +481,7 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
 #pragma unroll
                 for (int e = 0; e < EV; ++e) {
                     const int i = (v * VL + vl) * EV + e;
-                    if (i < hd) st[kStateHead + i] = acc[g][v * EV + e];
+                    if (i < hd) st[kStateHead + i] = e & 1 ? acc[g][(v * EV + e) / 2].y : acc[g][(v * EV + e) / 2].x;
                 }
         }
     }
@@ -862,10 +874,11 @@ cudaError_t run_fma_heads(AttnArgs a, int64_t n_rows, cudaStream_t st) {
     return launch_attend(kern, Shape::kWarps, smem, a, n_rows, st);
 }
 
-// Four query heads take the ring, one and two the registers, in us (B200):
-//   94 rows of 2511 keys, 16 heads over 2 of 64, f32       113 / 169
-//   7 rows of 1922 keys, 32 heads over 16 of 128, f32       46 / 40
-//   128 rows up to 8196 keys, 16 heads of 64, bf16         340 / 312 (1.98 GB: 6.3 TB/s)
+// Four query heads take the ring, one and two the registers.  Ring / registers
+// in us (B200):
+//   94 rows of 2511 keys, 16 heads over 2 of 64, f32       118 / 171
+//   7 rows of 1922 keys, 32 heads over 16 of 128, f32       47 / 39
+//   128 rows up to 8196 keys, 16 heads of 64, bf16         326 / 296 (1.98 GB: 6.7 TB/s)
 template <typename TC, int VL, int VPL>
 cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
     switch (group_chunk(a.group)) {
