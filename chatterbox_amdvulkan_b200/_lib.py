@@ -27,8 +27,8 @@ BIAS_NE0, BIAS_NE1 = 0, 1
 EFLAG_TOKEN_OOB, EFLAG_POS_OOB = 0x1, 0x2
 # error-word bits of the paged entry points and cbx_token_logprobs
 EFLAG_NO_PAGE, EFLAG_PAGE_OOB, EFLAG_LENGTH = 0x4, 0x8, 0x10
-# limits of the paged entry points and cbx_token_logprobs
-PAGED_MAX_REQS, LOGPROBS_MAX_TOP = 8192, 32
+# most alternatives of cbx_token_logprobs
+LOGPROBS_MAX_TOP = 32
 # bits of the library's device error word (cbx_device_errors)
 DEVERR_WAIT_TIMEOUT = 0x1
 

@@ -109,13 +109,8 @@ __device__ __forceinline__ void grid_dep_launch() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Thread-block clusters: this CTA's rank, and the barrier of all the cluster's
-// threads, which also orders their global and (distributed) shared accesses.
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
+// The barrier of all threads of a thread-block cluster, which also orders their
+// global and (distributed) shared memory accesses.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

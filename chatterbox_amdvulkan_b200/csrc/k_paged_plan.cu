@@ -22,9 +22,11 @@
 //    barrier cannot wait for a CTA that is not running) pushes the released
 //    pages, then the cluster barrier makes them visible and ends all reads of
 //    what is overwritten.
-// Measured with new outputs: 512 requests of 513 blocks, 262,656 pages: 20.3 us
-// with the cluster alone, 5.1 us with the grid; 64 requests, 65,536 rows: 11.7
-// and 4.3 us.
+// Measured: 512 requests of 513 blocks, 262,656 pages, one token each: 5.1 us
+// with new outputs (20.3 us with the cluster), 7.0 us in place; 64 requests,
+// 65,536 rows: 4.1 us (11.7) and 10.6 us; 64 requests, one token each, in place:
+// 4.1 us.  (Four rows to a thread, with 16-byte stores, was slower: 8.2 and 6.5
+// us with new outputs.)
 #include "cbx_common.cuh"
 
 namespace cbx {
@@ -212,23 +214,29 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a) {
 
     // Tables and counts.  In place the kept entries stay; those behind the last
     // page become -1 whatever they held.
-    const int64_t entries = (int64_t)B * a.max_blocks;
-    for (int64_t i = me; i < entries; i += all) {
-        const int b = (int)((uint32_t)i / (uint32_t)a.max_blocks), j = (int)(i - (int64_t)b * a.max_blocks);
-        const int need = s_need[b], have = s_have[b], keep = need < have ? need : have;
-        if (IN_PLACE && a.table == a.table_in && j < keep) continue;
+    auto write_entry = [&](int b, int j, int need, int have) {
+        const int64_t i = (int64_t)b * a.max_blocks + j;
         const int left = top - s_pop[b];  // pages on the stack when b's turn comes
         int page = -1;
-        if (j < need) {
-            if (j < have) page = a.table_in[i];
-            else if (j - have < left) page = on_stack(left - 1 - (j - have));
-            else {
-                a.table[i] = -1;  // none is left
-                continue;
-            }
+        if (j < need && (j < have || j - have < left)) {
+            page = j < have ? a.table_in[i] : on_stack(left - 1 - (j - have));
             if (page < 0 || page >= a.n_pages) flags |= CBX_EFLAG_PAGE_OOB;
         }
         a.table[i] = page;
+    };
+    if (IN_PLACE) {  // a warp takes a row: most of its entries are stores of -1
+        const int lane = tid & 31, warps = (int)(all / 32);
+        for (int b = (int)(me / 32); b < B; b += warps) {
+            const int need = s_need[b], have = s_have[b];
+            for (int j = (a.table == a.table_in ? min(need, have) : 0) + lane; j < a.max_blocks; j += 32)
+                write_entry(b, j, need, have);
+        }
+    } else {
+        const int64_t entries = (int64_t)B * a.max_blocks;
+        for (int64_t i = me; i < entries; i += all) {
+            const int b = (int)((uint32_t)i / (uint32_t)a.max_blocks);
+            write_entry(b, (int)(i - (int64_t)b * a.max_blocks), s_need[b], s_have[b]);
+        }
     }
     for (int64_t b = me; b < B; b += all) {
         const int need = s_need[b], have = s_have[b], left = top - s_pop[b];

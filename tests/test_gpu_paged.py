@@ -131,6 +131,21 @@ def test_plan_without_requests_and_with_the_most(ops):
     check_plan(p, plan_ref(lens, lens, st["table"], st["n_blocks"], st["free"], B * 4, 16, sum(lens)))
 
 
+def test_plan_writes_only_its_rows(ops):
+    """Buffers that start and end at odd places: what lies around them stays."""
+    lens, new = [9, 0, 3, 30], [2, 0, 3, 17]
+    st = pool(4, 4, 16)
+    for off, rows in ((0, 22), (1, 25), (2, 23), (3, 40)):
+        bufs = [torch.full((64,), 77, dtype=torch.int32, device="cuda") for _ in range(4)]
+        state = [torch.empty(n, dtype=torch.int32, device="cuda") for n in (5, 16, 4, 16, 1)]
+        p = ops.paged_plan(ints(lens), ints(st["table"]), ints(st["n_blocks"]), ints(st["free"]), ints([16]), 8,
+                           n_new=ints(new), max_rows=rows, out=[b[off:off + rows] for b in bufs] + state)
+        check_plan(p._replace(block_table=p.block_table.view(4, 4)),
+                   plan_ref(lens, new, st["table"], st["n_blocks"], st["free"], 16, 8, rows))
+        for b in bufs:
+            assert (b[:off] == 77).all() and (b[off + rows:] == 77).all()
+
+
 # ----------------------------------------------------------------- append --
 
 def rounded(x, t):
