@@ -490,9 +490,14 @@ k_token_logprobs(LogprobArgs a) {
         const float log_s = log2f(s);
         // ln sum e^(x - m): the sums refer to ref, which m log2 e is below by the FMA's value.
         const float ln_s = (log_s - (huge ? 0.0f : fmaf(m, kLog2e, -ref))) * kLn2;
-        auto log_prob = [&](float x) { return bad ? (float)NAN : (x - m) - ln_s; };
+        // The sum's rounding may put a value that is 0 but for it 2^-24 on the wrong side of 0.
+        auto log_prob = [&](float x) {
+            const float v = (x - m) - ln_s;
+            return bad ? (float)NAN : v > 0.0f ? 0.0f : v;  // NaN (no token) stays
+        };
         if (tid == 0) {
-            if (a.entropy) a.entropy[r] = bad ? NAN : (log_s - t / s) * kLn2;
+            const float h = (log_s - t / s) * kLn2;
+            if (a.entropy) a.entropy[r] = bad ? (float)NAN : h < 0.0f ? 0.0f : h;
             if (a.logprob) {
                 if (tok < -1 || tok >= row.V) atomicOr(a.err, CBX_EFLAG_TOKEN_OOB);
                 a.logprob[r] = log_prob(to_f(x_tok));  // NaN without a token

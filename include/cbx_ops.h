@@ -543,7 +543,8 @@ CBX_API int64_t cbx_paged_decode_attention_workspace(int64_t n_rows, int64_t n_h
  * vocab), of `type` F32 / F16 / BF16; sums in f32; all outputs f32 / int32.
  * 0 <= top_k <= min(vocab, CBX_LOGPROBS_MAX_TOP).  tokens and logprob may both
  * be NULL, entropy may be NULL, top_ids / top_logprobs are needed for
- * top_k > 0 only.  A logit of -inf is a token of probability 0.  A row with a
+ * top_k > 0 only.  No log probability is above 0, no entropy below it.
+ * A logit of -inf is a token of probability 0.  A row with a
  * NaN, a +inf, or nothing but -inf has no distribution: its values are NaN,
  * its top_ids still the order of the logits (NaN above all, by rising j).  A
  * token outside [0, vocab) gives logprob NaN and ORs CBX_EFLAG_TOKEN_OOB into

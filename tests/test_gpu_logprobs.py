@@ -49,6 +49,20 @@ def test_logprobs(ops, t, N, V, k):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V", [1, 2, 300, 6563])
+def test_logprobs_of_one_sure_token(ops, t, V):
+    """One token takes all: its log probability is 0 up to rounding and never above, the entropy never below."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(2000, V, generator=g, device="cuda")
+    tokens = torch.randint(0, V, (2000,), generator=g, device="cuda", dtype=torch.int32)
+    x.scatter_(1, tokens.long()[:, None], x.gather(1, tokens.long()[:, None]) + 40.0 * (V > 1))
+    x = x.to(t)
+    got = ops.token_logprobs(x, tokens, top_k=1)
+    check(got, x, tokens, 1)
+    assert (got.logprobs <= 0).all() and (got.top_logprobs <= 0).all() and (got.entropy >= 0).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_logprobs_strided_and_shifted_rows(ops, t):
     """Rows that start at every place within 16 bytes; a padded vocabulary whose tail must not count."""
     for off in range(9):
