@@ -13,10 +13,10 @@
 // Bound by HBM: each key and value is read once and takes 2 FMAs per query
 // head.  Two kernels, both with whole tiles of keys and values in flight per
 // warp and no CTA barrier in the loop:
-//  - k_attend_fma: one or two query heads per kv head, or an f32 cache.  A key
-//    row of one kv head is VL 16-byte vectors, one per lane, so a warp reads
-//    32 / VL keys per load instruction.  f32 FMAs.
-//  - k_attend_mma: 16-bit caches and more query heads per kv head, where the
+//  - k_attend_fma: one query head per kv head, two with an f32 cache, or heads
+//    of more than 128 elements.  A key row of one kv head is VL 16-byte vectors,
+//    one per lane, so a warp reads 32 / VL keys per load instruction.  f32 FMAs.
+//  - k_attend_mma, k_attend_mma_f32: more query heads per kv head, where the
 //    FMAs and the conversions to f32 would bound it.  mma.sync of 16 rows: the
 //    up to 8 query heads of a kv head, twice.
 //
@@ -229,6 +229,12 @@ __device__ __forceinline__ uint4 lds16(uint32_t p) {
     return v;
 }
 
+__device__ __forceinline__ float lds_f32(uint32_t p) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+    return v;
+}
+
 // The elements of a 16-byte vector as pairs of f32, for the packed FMAs.
 template <typename TC, int N>
 __device__ __forceinline__ void pairs_of(uint4 w, float2 (&f)[N], TC) {
@@ -257,6 +263,7 @@ struct Fma {
     static constexpr int kStages = 3;
     static constexpr int kRingBytes = RING ? kStages * 2 * kLoads * VPL * 512 : 0;  // of a warp
 };
+constexpr int kRingStep = 16;  // keys of a step with the ring, which takes head_dim above 128 only
 
 template <typename TC, int VL, int VPL, int G, bool RING>
 __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(AttnArgs a) {
@@ -264,6 +271,7 @@ __global__ void __launch_bounds__(Fma<VL, VPL, RING>::kWarps * 32) k_attend_fma(
     constexpr int EV = Vec<TC>::n;        // elements per 16-byte vector
     constexpr int EL = EV * VPL;          // elements of the head per lane
     constexpr int U = Shape::kLoads, KPL = Shape::kKeysPerLoad, TILE = Shape::kTile, step = Shape::kStep;
+    static_assert(!RING || step == kRingStep, "choose_splits counts the ring's steps");
     extern __shared__ __align__(128) float smem[];  // rings, then states
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vl = lane % VL, kg = lane / VL;
@@ -743,6 +751,263 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
     finish<kMmaWarps, kMmaHeads>(a, w, smem);
 }
 
+__device__ __forceinline__ void mma1688(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two tf32 terms of f32 values.  By truncation (2.5 instructions a value): 11
+// bits each, so less than 2^-21 of the value is lost, and nothing overflows.
+// Rounded: at most 2^-24 is lost, but cvt takes several instructions (with it for
+// all values the first two cases below took 57.9 and 157 us): for the query, split
+// once, and P, of which a tile has few.
+__device__ __forceinline__ void tf32_rounded(float x, uint32_t* t) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(t[0]) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(t[1]) : "f"(x - __uint_as_float(t[0])));
+}
+__device__ __forceinline__ void tf32_terms(float x, float y, uint32_t (&t)[2][2]) {
+    t[0][0] = __float_as_uint(x) & 0xffffe000u;
+    t[1][0] = __float_as_uint(y) & 0xffffe000u;
+    const float2 r = __ffma2_rn(make_float2(__uint_as_float(t[0][0]), __uint_as_float(t[1][0])), pair(-1.0f), make_float2(x, y));
+    t[0][1] = __float_as_uint(r.x) & 0xffffe000u;
+    t[1][1] = __float_as_uint(r.y) & 0xffffe000u;
+}
+
+// Shape of the f32 form: KEYS per warp and step (16 of up to 64 elements, 8 of
+// more), two tiles of a warp in shared memory, and CTAs per SM, by registers.
+// In us (B200), with 2 / 3 / 4 CTAs per SM:
+//   94 rows of 2511 keys, 16 heads over 2 of 64     61.6 / 49.8 / 61.3 (241 MB: 4.8 TB/s)
+//   40 rows of 4000 keys, 32 heads over 4 of 128    141 / 158 / 233 (655 MB: 4.7 TB/s)
+//   64 rows of 2000 keys, 16 heads over 4 of 32     34.3 / 34.3 / 30.6
+// Three tiles, or 8 keys of 64 elements or 16 of 128, were no faster.
+template <int HD>
+struct MmaF32 {
+    static constexpr int kKeys = HD <= 64 ? 16 : 8;
+    static constexpr int kStages = 2;
+    static constexpr int kPerSM = HD <= 32 ? 4 : HD <= 64 ? 3 : 2;
+    static constexpr int kTileBytes = kKeys * HD * 4;            // of K, and of V
+    static constexpr int kRingBytes = kStages * 2 * kTileBytes;  // of a warp
+    static constexpr int kStep = kKeys * kMmaWarps;
+};
+
+// The same for f32 caches, by m16n8k8 products of tf32: every value is the sum of
+// two tf32 terms, rows 0-7 of the first operand are the heads' first terms, rows
+// 8-15 their second ones, and the second operand's terms take a product each.
+// Lanes read 16 bytes at a time and split them in registers:
+//   K: elements 4t .. 4t + 3 of 16 are k = t and t + 4 of two products (the query's
+//     elements are taken in the same order);
+//   V: keys 2t and 2t + 1 of 8 are k = t and t + 4, as the scores lie, and elements
+//     4g .. 4g + 3 of 32 are column g of four products.
+// The vectors of a row are permuted so that the 8 lanes of a shared-memory
+// access meet no bank twice.  The terms of an infinite key are NaN: a tile with a
+// NaN score is scored again by f32 FMAs.
+// Against f32 FMAs with four heads a CTA, in us (B200): 94 rows of 2511 keys, 16
+// heads over 2 of 64, 50 / 99, 8 heads over 2, 48 / 82; 40 rows of 4000 keys, 32 heads
+// over 4 of 128, 141 / 281; 300 rows of 500 keys, 64 heads over 4 of 64, 110 / 207.
+// With two heads the FMAs are faster: 40 rows, 8 over 4 of 128, 128 / 105.  Three
+// bf16 terms a value, which lose nothing, take 11 instructions a pair: 55.6 and 175
+// us for the first and third.  What bounds it is issue: a value is split by every
+// CTA that reads it, at 2.5 instructions.
+template <int HD>
+__global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_mma_f32(AttnArgs a) {
+    using Shape = MmaF32<HD>;
+    constexpr int KS = HD / 16, VECS = HD / 4, KEYS = Shape::kKeys, NT = KEYS / 8, STAGES = Shape::kStages;
+    constexpr int step = Shape::kStep;
+    extern __shared__ __align__(128) float smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int hd = a.head_dim, vecs = hd / 4;
+    grid_dep_wait();
+    grid_dep_launch();
+    Work w(a, kMmaHeads, step);
+
+    float o[HD / 8][4] = {};  // [4 b + c]: elements 32 b + 4 n + c, n = 2t and 2t + 1
+    float m = -INFINITY, l = 0.0f;  // head g
+    const char* kbase = static_cast<const char*>(a.ck) + (int64_t)w.kvh * hd * 4;
+    const char* vbase = static_cast<const char*>(a.cv) + (int64_t)w.kvh * hd * 4;
+    const int64_t row_bytes = a.kv_dim * 4;
+    constexpr uint32_t kTileBytes = Shape::kTileBytes;
+    const uint32_t ring = smem_addr(smem) + warp * Shape::kRingBytes;
+    auto k_cell = [](int r, int c) { return (uint32_t)(r * HD * 4 + ((c ^ ((r & 1) << 2)) << 4)); };
+    auto v_cell = [](int r, int c) { return (uint32_t)(r * HD * 4 + ((c ^ (r & 7)) << 4)); };
+
+    // Puts the tile at t0 in a stage; returns which of its keys are there.
+    auto fetch = [&](int64_t t0, int stage, int slot) {
+        const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & ((1u << KEYS) - 1);
+        if (t0 < w.hi) {
+            constexpr int kRows = 32 / VECS;  // rows per instruction
+            const int r0 = lane / VECS, c = lane % VECS;
+            const uint32_t dst = ring + stage * 2 * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < KEYS / kRows; ++i) {
+                const int r = i * kRows + r0;
+                const int s = __shfl_sync(0xffffffffu, slot, r);
+                const bool in = s >= 0 && c < vecs;
+                const int64_t off = in ? s * row_bytes + c * 16 : 0;
+                copy16(dst + k_cell(r, c), kbase + off, in);
+                copy16(dst + kTileBytes + v_cell(r, c), vbase + off, in);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return there;
+    };
+
+    const int64_t first = w.lo + (int64_t)warp * KEYS;
+    const int my_key = lane & (KEYS - 1);
+    uint64_t there = 0;  // 16 bits for each tile on its way, the oldest on top
+    int entries[STAGES], slot = -1;
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) entries[s] = w.entry(a, first + (int64_t)s * step + my_key);
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+        slot = w.row_of(a, entries[s], first + (int64_t)s * step + my_key);
+        if (s < STAGES - 1) there = there << 16 | fetch(first + (int64_t)s * step, s, slot);
+    }
+    // Head g's query.
+    uint32_t qf[KS][2][4];
+    with_type(a.q, a.q_type, [&](auto* p) {
+        p += (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = 16 * s + 4 * t + 2 * h;  // head_dim is even: both or neither
+                const bool in = g < w.heads && i < hd;
+                tf32_rounded(in ? to_f(p[i]) : 0.0f, qf[s][h]);
+                tf32_rounded(in ? to_f(p[i + 1]) : 0.0f, qf[s][h] + 2);
+            }
+    });
+    int stage = 0;
+    for (int64_t t0 = first; t0 < w.hi; t0 += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();  // all lanes' copies have landed, and all have left the stage that is filled next
+        int next = stage + STAGES - 1;
+        if (next >= STAGES) next -= STAGES;
+        there = there << 16 | fetch(t0 + (int64_t)(STAGES - 1) * step, next, slot);
+        slot = w.find(a, t0 + (int64_t)STAGES * step + my_key);
+        const uint32_t keys = (uint32_t)(there >> (16 * (STAGES - 1))) & 0xffffu;
+        const uint32_t kt = ring + stage * 2 * kTileBytes, vt = kt + kTileBytes;
+        if (++stage == STAGES) stage = 0;
+
+        // Scores of head g: keys 8n + 2t, 8n + 2t + 1.
+        float s[NT][2];
+        bool odd = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float c[2][4] = {};  // the large products, the small ones
+#pragma unroll
+            for (int q = 0; q < KS; ++q) {
+                const uint4 x = lds16(kt + k_cell(n * 8 + g, 4 * q + t));
+                uint32_t b[2][2][2];
+                tf32_terms(__uint_as_float(x.x), __uint_as_float(x.y), b[0]);
+                tf32_terms(__uint_as_float(x.z), __uint_as_float(x.w), b[1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) mma1688(c[k], qf[q][h], b[h][0][k], b[h][1][k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                s[n][k] = (c[0][k] + c[0][k + 2]) + (c[1][k] + c[1][k + 2]);
+                odd |= s[n][k] != s[n][k];
+            }
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+            with_type(a.q, a.q_type, [&](auto* p) {
+                p += (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
+                for (int n = 0; n < 2 * NT; ++n) {
+                    const int r = (n >> 1) * 8 + 2 * t + (n & 1);
+                    float sum = 0.0f;
+                    for (int i = 0; i < hd && g < w.heads; ++i)
+                        sum = fmaf(to_f(p[i]), lds_f32(kt + k_cell(r, i >> 2) + (i & 3) * 4), sum);
+#pragma unroll
+                    for (int k = 0; k < 2 * NT; ++k)
+                        if (k == n) s[k >> 1][k & 1] = sum;
+                }
+            });
+        }
+        float best = m;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bool in = keys >> (8 * n + 2 * t + k) & 1;
+                s[n][k] = in ? s[n][k] * a.scale_log2 : -INFINITY;
+                best = fmaxf(best, s[n][k]);
+            }
+        if (__any_sync(0xffffffffu, best > m)) {
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+            const float c = rescale(m, best);
+            m = best;
+            l *= c;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[j][k] *= c;
+        }
+        uint32_t pf[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float p0 = s[n][0] == -INFINITY ? 0.0f : ex2_approx(s[n][0] - m);
+            const float p1 = s[n][1] == -INFINITY ? 0.0f : ex2_approx(s[n][1] - m);
+            l += p0 + p1;
+            tf32_rounded(p0, pf[n]);
+            tf32_rounded(p1, pf[n] + 2);
+        }
+#pragma unroll
+        for (int b = 0; b < HD / 32; ++b) {
+            // The products truncate what they add up: the first terms' sums start
+            // anew each tile and are added with rounding (2.5 % of the time; 12 rows
+            // of 4693 keys, 80 heads over 16 of 72: off by 1.1e-6, not 6.4e-6).
+            float d[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                d[c][0] = d[c][1] = 0.0f;
+                d[c][2] = o[4 * b + c][2];
+                d[c][3] = o[4 * b + c][3];
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint4 x = lds16(vt + v_cell(8 * n + 2 * t, 8 * b + g)), y = lds16(vt + v_cell(8 * n + 2 * t + 1, 8 * b + g));
+                const uint32_t v[4][2] = {{x.x, y.x}, {x.y, y.y}, {x.z, y.z}, {x.w, y.w}};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t f[2][2];
+                    tf32_terms(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), f);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) mma1688(d[c], pf[n], f[0][k], f[1][k]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                o[4 * b + c][0] += d[c][0];
+                o[4 * b + c][1] += d[c][1];
+                o[4 * b + c][2] = d[c][2];
+                o[4 * b + c][3] = d[c][3];
+            }
+        }
+    }
+    if (w.flags) atomicOr(a.err, w.flags);
+
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the states take the rings' place
+    float* st = smem + (warp * kMmaHeads + g) * state_floats(hd);
+    if (t == 0) {
+        st[0] = m;
+        st[1] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int e = 32 * (j >> 2) + 4 * (2 * t + k) + (j & 3);
+            if (e < hd) st[kStateHead + e] = o[j][k] + o[j][k + 2];
+        }
+    finish<kMmaWarps, kMmaHeads>(a, w, smem);
+}
+
 // Joins the splits' states of one row and head: first the weight of each split,
 // then the values, 16 bytes a load, the splits shared by the threads so that a
 // thread's few loads travel together (one thread for all splits of an element
@@ -806,7 +1071,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttnArgs a) {
 // Query heads of a CTA.
 int group_chunk(int group) { return group >= 3 ? 4 : group; }
 bool use_mma(int cache_type, int group, int head_dim) {
-    return cache_type != CBX_TYPE_F32 && group > 1 && head_dim <= 128;
+    return head_dim <= 128 && group >= (cache_type == CBX_TYPE_F32 ? 3 : 2);
 }
 
 struct Splits {
@@ -830,11 +1095,19 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
     const bool mma = use_mma(cache_type, group, (int)head_dim);
     const int gc = mma ? kMmaHeads : group_chunk(group);
     const int64_t vecs = head_dim * type_size(cache_type) / 16;
-    const int64_t step = mma ? kMmaTile * kMmaWarps
-                       : 8 * (vecs <= 4 ? 32 : vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
-    // CTAs per SM by registers (and shared memory): the tensor-core kernel's f32
-    // queries take 3 terms, and so more registers, on bf16 caches only.
-    const int64_t resident = (int64_t)num_sms() * (mma && head_dim <= 64 ? (cache_type == CBX_TYPE_F16 ? 4 : 3) : 2);
+    const bool f32 = cache_type == CBX_TYPE_F32;
+    int64_t step, per_sm;  // CTAs per SM by registers and shared memory
+    if (mma && f32) {
+        step = head_dim <= 32 ? MmaF32<32>::kStep : head_dim <= 64 ? MmaF32<64>::kStep : MmaF32<128>::kStep;
+        per_sm = head_dim <= 32 ? MmaF32<32>::kPerSM : head_dim <= 64 ? MmaF32<64>::kPerSM : MmaF32<128>::kPerSM;
+    } else if (mma) {  // f32 queries take 3 terms, and so more registers, on bf16 caches only
+        step = kMmaTile * kMmaWarps;
+        per_sm = head_dim > 64 ? 2 : cache_type == CBX_TYPE_F16 ? 4 : 3;
+    } else {
+        step = group > 2 ? kRingStep : 8 * (vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
+        per_sm = 2;
+    }
+    const int64_t resident = num_sms() * per_sm;
     const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
     if (ctas >= 8 * resident) return {1, false};
     const int64_t steps = (max_keys + step - 1) / step;
@@ -874,18 +1147,20 @@ cudaError_t run_fma_heads(AttnArgs a, int64_t n_rows, cudaStream_t st) {
     return launch_attend(kern, Shape::kWarps, smem, a, n_rows, st);
 }
 
-// Four query heads take the ring, one and two the registers.  Ring / registers
-// in us (B200):
-//   94 rows of 2511 keys, 16 heads over 2 of 64, f32       118 / 171
-//   7 rows of 1922 keys, 32 heads over 16 of 128, f32       47 / 39
+// Heads of more than 128 elements, four at a time, take the ring, others the
+// registers.  Ring / registers / registers with two at a time, in us (B200):
+//   40 rows of 4000 keys, 32 heads over 4 of 160, f32      426 / 477 / 688
+//   94 rows of 2511 keys, 16 heads over 2 of 256, bf16     242 / 348 / 429
+//   30 rows of 2511 keys, 8 heads over 2 of 256, f32       99 / 74 / 108
 //   128 rows up to 8196 keys, 16 heads of 64, bf16         326 / 296 (1.98 GB: 6.7 TB/s)
 template <typename TC, int VL, int VPL>
 cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
-    switch (group_chunk(a.group)) {
-        case 1: return run_fma_heads<TC, VL, VPL, 1, false>(a, n_rows, st);
-        case 2: return run_fma_heads<TC, VL, VPL, 2, false>(a, n_rows, st);
-        default: return run_fma_heads<TC, VL, VPL, 4, true>(a, n_rows, st);
-    }
+    constexpr bool wide = VL * VPL * Vec<TC>::n > 128;  // heads that the tensor-core kernels do not take
+    if constexpr (wide)
+        if (a.group > 2) return run_fma_heads<TC, VL, VPL, 4, true>(a, n_rows, st);
+    if constexpr (wide || sizeof(TC) == 4)
+        if (a.group == 2) return run_fma_heads<TC, VL, VPL, 2, false>(a, n_rows, st);
+    return run_fma_heads<TC, VL, VPL, 1, false>(a, n_rows, st);
 }
 
 template <typename T, int HD>
@@ -900,12 +1175,29 @@ cudaError_t run_mma(AttnArgs a, int64_t n_rows, bool same_type, cudaStream_t st)
     return launch_attend(kern, kMmaWarps, smem, a, n_rows, st);
 }
 
+template <int HD>
+cudaError_t run_mma_f32(AttnArgs a, int64_t n_rows, cudaStream_t st) {
+    a.chunks = (a.group + kMmaHeads - 1) / kMmaHeads;
+    const size_t states = sizeof(float) * (kMmaWarps + 1) * kMmaHeads * state_floats(a.head_dim);
+    const size_t rings = (size_t)kMmaWarps * MmaF32<HD>::kRingBytes;
+    const size_t smem = states > rings ? states : rings;
+    auto kern = k_attend_mma_f32<HD>;
+    if (!smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
+    return launch_attend(kern, kMmaWarps, smem, a, n_rows, st);
+}
+
 template <typename TC>
 cudaError_t run_head(const AttnArgs& a, int cache_type, int64_t n_rows, cudaStream_t st) {
     if constexpr (sizeof(TC) == 2) {
         if (use_mma(cache_type, a.group, a.head_dim))
             return a.head_dim <= 64 ? run_mma<TC, 64>(a, n_rows, a.q_type == cache_type, st)
                                     : run_mma<TC, 128>(a, n_rows, a.q_type == cache_type, st);
+    }
+    if constexpr (sizeof(TC) == 4) {
+        if (use_mma(cache_type, a.group, a.head_dim))
+            return a.head_dim <= 32   ? run_mma_f32<32>(a, n_rows, st)
+                   : a.head_dim <= 64 ? run_mma_f32<64>(a, n_rows, st)
+                                      : run_mma_f32<128>(a, n_rows, st);
     }
     const int vecs = (a.head_dim + Vec<TC>::n - 1) / Vec<TC>::n;
     if (vecs <= 4) return run_fma<TC, 4, 1>(a, n_rows, st);

@@ -495,11 +495,14 @@ CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_r
  * apart (0 = dense; out is dense); caches as in cbx_qkv_kv_append_paged with
  * kv_dim = n_kv_heads * head_dim, of cache_type; table [n_reqs][max_blocks].
  * q_type and cache_type: any of F32 / F16 / BF16.  Products, softmax and sums
- * are f32; out is rounded once.  Several rows may name one request (the tokens
- * of a prefill chunk or of a speculated continuation, each with its length).
- * A row of length 0 gives zeros and lse -inf, and so does one whose scores are
- * all -inf.  Infinities and NaN in q or below the length in the keys and values
- * give what the formula gives, or NaN.  lse (f32 [n_rows][n_heads]) may be NULL.  Keys at and behind the length are not read, whatever the memory
+ * are f32 (the tensor cores' products of an f32 cache, for 3 and more query
+ * heads per kv head, take keys and values to 2^-21); out is rounded once.
+ * Several rows may name one request (the tokens of a prefill chunk or of a
+ * speculated continuation, each with its length).  A row of length 0 gives zeros
+ * and lse -inf, and so does one whose scores are all -inf.  Infinities and NaN in
+ * q or below the length in the keys and values give what the formula gives, or
+ * NaN.  lse (f32 [n_rows][n_heads]) may be NULL.
+ * Keys at and behind the length are not read, whatever the memory
  * holds.  Keys whose table entry is outside [0, n_pages) are left out of the
  * sums and raise CBX_EFLAG_PAGE_OOB, a row_reqs entry outside [0, n_reqs) does
  * too (the row counts as empty); a length above max_blocks * page_size or below

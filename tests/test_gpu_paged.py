@@ -338,6 +338,18 @@ def test_attention_scores_of_minus_infinity(ops, qt, ct, H, Hk):
     assert not out[2].any() and (lse[2] == -math.inf).all()
 
 
+@pytest.mark.parametrize("H,Hk,hd", [(3, 1, 24), (8, 2, 32), (12, 1, 40), (16, 2, 64), (17, 1, 96), (4, 1, 128)])
+@pytest.mark.parametrize("qt", [F32, BF16])
+@pytest.mark.parametrize("kpow,vpow", [(0, 0), (60, -100), (-60, 110)])
+def test_attention_f32_caches_of_any_magnitude(ops, H, Hk, hd, qt, kpow, vpow):
+    """Keys and values far from 1, scores of a like size (300 values of 2^110 sum to less than 2^128)."""
+    q, ck, cv, table, n = make([300, 33, 1], H, Hk, hd, 16, qt, F32, hd)
+    q, ck = (q.float() * 2.0 ** -kpow).to(qt), ck * 2.0 ** kpow
+    cv = cv.clamp(-0.9, 0.9) * 2.0 ** vpow
+    a = (q, ck, cv, table, n)
+    check_attention(ops.paged_decode_attention(*a), attention_ref(*a))
+
+
 def test_attention_many_rows_of_one_request(ops):
     """row_reqs: the tokens of a prefill chunk, each row with its own length, and unordered requests."""
     q, ck, cv, table, n = make([50, 20, 33], 4, 2, 64, 16, F32, F16, 7)
