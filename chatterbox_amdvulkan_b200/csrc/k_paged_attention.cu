@@ -806,8 +806,9 @@ struct MmaF32 {
 // over 4 of 128, 141 / 281; 300 rows of 500 keys, 64 heads over 4 of 64, 110 / 207.
 // With two heads the FMAs are faster: 40 rows, 8 over 4 of 128, 128 / 105.  Three
 // bf16 terms a value, which lose nothing, take 11 instructions a pair: 55.6 and 175
-// us for the first and third.  What bounds it is issue: a value is split by every
-// CTA that reads it, at 2.5 instructions.
+// us for the first and third.  What bounds it is latency: of the splits and of
+// products that wait for one another, at 12 warps an SM (issue slots 47 % busy,
+// tensor pipe 32 %); the registers leave no room for more.
 template <int HD>
 __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_mma_f32(AttnArgs a) {
     using Shape = MmaF32<HD>;
