@@ -546,7 +546,8 @@ __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tile
     return kMmaStages * 2 * kMmaTile * HD * 2;
 }
 
-// S = Q K^T and O = P V by m16n8k16 products.  Rows 0-7 of the first operand
+// S = Q K^T and O = P V by m16n8k16 products, for heads of up to W elements; the
+// rows of the rings are HD elements long.  Rows 0-7 of the first operand
 // are the first 16-bit term of the 8 heads' values, rows 8-15 the second: Q and
 // P are f32 values written as sums of 16-bit ones, so that the products are as
 // exact as f32 ones where the result is.
@@ -564,10 +565,10 @@ __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tile
 // ring (both with the first form of the join; 50 us, 5.4 TB/s, now).  f32 FMAs
 // with 4 heads a CTA took 107 us there.  The 16-byte vectors of a row are permuted by the
 // row's number, which keeps ldmatrix free of bank conflicts.
-template <typename T, int HD, int QT, int PT>
+template <typename T, int HD, int W, int QT, int PT>
 __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
-    constexpr int KS = HD / 16;    // products over the head
-    constexpr int VECS = HD / 8;   // 16-byte vectors of a row in the ring
+    constexpr int KS = W / 16;    // products over the head
+    constexpr int VECS = W / 8;   // 16-byte vectors of a row
     constexpr int step = kMmaTile * kMmaWarps;
     extern __shared__ __align__(128) float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -588,8 +589,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
     auto fetch = [&](int64_t t0, int stage, int slot) {
         const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
         if (t0 < w.hi) {
-            constexpr int kRows = 32 / VECS;  // rows per instruction
-            const int r0 = lane / VECS, c = lane % VECS;
+            constexpr int kCells = HD / 8, kRows = 32 / kCells;  // rows per instruction
+            const int r0 = lane / kCells, c = lane % kCells;
             const uint32_t dst = ring + stage * 2 * kTileBytes;
 #pragma unroll
             for (int i = 0; i < kMmaTile / kRows; ++i) {
@@ -804,15 +805,17 @@ struct MmaF32 {
 // Against f32 FMAs with four heads a CTA, in us (B200): 94 rows of 2511 keys, 16
 // heads over 2 of 64, 50 / 99, 8 heads over 2, 48 / 82; 40 rows of 4000 keys, 32 heads
 // over 4 of 128, 141 / 281; 300 rows of 500 keys, 64 heads over 4 of 64, 110 / 207.
-// With two heads the FMAs are faster: 40 rows, 8 over 4 of 128, 128 / 105.  Three
+// With two heads the FMAs are faster: 40 rows, 8 over 4 of 128, 128 / 105; and with
+// a few keys, as the long code has to be fetched: 6 rows of 13 keys, 16 over 2 of
+// 128, 6.9 / 4.8 (the host knows the tables' size only, not the lengths).  Three
 // bf16 terms a value, which lose nothing, take 11 instructions a pair: 55.6 and 175
 // us for the first and third.  What bounds it is latency: of the splits and of
 // products that wait for one another, at 12 warps an SM (issue slots 47 % busy,
 // tensor pipe 32 %); the registers leave no room for more.
-template <int HD>
+template <int HD, int W>
 __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_mma_f32(AttnArgs a) {
     using Shape = MmaF32<HD>;
-    constexpr int KS = HD / 16, VECS = HD / 4, KEYS = Shape::kKeys, NT = KEYS / 8, STAGES = Shape::kStages;
+    constexpr int KS = W / 16, KEYS = Shape::kKeys, NT = KEYS / 8, STAGES = Shape::kStages;
     constexpr int step = Shape::kStep;
     extern __shared__ __align__(128) float smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -821,7 +824,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_m
     grid_dep_launch();
     Work w(a, kMmaHeads, step);
 
-    float o[HD / 8][4] = {};  // [4 b + c]: elements 32 b + 4 n + c, n = 2t and 2t + 1
+    float o[W / 8][4] = {};  // [4 b + c]: elements 32 b + 4 n + c, n = 2t and 2t + 1
     float m = -INFINITY, l = 0.0f;  // head g
     const char* kbase = static_cast<const char*>(a.ck) + (int64_t)w.kvh * hd * 4;
     const char* vbase = static_cast<const char*>(a.cv) + (int64_t)w.kvh * hd * 4;
@@ -835,8 +838,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_m
     auto fetch = [&](int64_t t0, int stage, int slot) {
         const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0) & ((1u << KEYS) - 1);
         if (t0 < w.hi) {
-            constexpr int kRows = 32 / VECS;  // rows per instruction
-            const int r0 = lane / VECS, c = lane % VECS;
+            constexpr int kCells = HD / 4, kRows = 32 / kCells;  // rows per instruction
+            const int r0 = lane / kCells, c = lane % kCells;
             const uint32_t dst = ring + stage * 2 * kTileBytes;
 #pragma unroll
             for (int i = 0; i < KEYS / kRows; ++i) {
@@ -942,7 +945,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_m
             m = best;
             l *= c;
 #pragma unroll
-            for (int j = 0; j < HD / 8; ++j)
+            for (int j = 0; j < W / 8; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[j][k] *= c;
         }
@@ -956,7 +959,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_m
             tf32_rounded(p1, pf[n] + 2);
         }
 #pragma unroll
-        for (int b = 0; b < HD / 32; ++b) {
+        for (int b = 0; b < W / 32; ++b) {
             // The products truncate what they add up: the first terms' sums start
             // anew each tile and are added with rounding (2.5 % of the time; 12 rows
             // of 4693 keys, 80 heads over 16 of 72: off by 1.1e-6, not 6.4e-6).
@@ -1000,7 +1003,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, MmaF32<HD>::kPerSM) k_attend_m
         st[1] = l;
     }
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j)
+    for (int j = 0; j < W / 8; ++j)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int e = 32 * (j >> 2) + 4 * (2 * t + k) + (j & 3);
@@ -1164,41 +1167,46 @@ cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
     return run_fma_heads<TC, VL, VPL, 1, false>(a, n_rows, st);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int W>
 cudaError_t run_mma(AttnArgs a, int64_t n_rows, bool same_type, cudaStream_t st) {
     constexpr bool bf16 = __is_same(T, __nv_bfloat16);
     a.chunks = (a.group + kMmaHeads - 1) / kMmaHeads;
     const size_t states = sizeof(float) * (kMmaWarps + 1) * kMmaHeads * state_floats(a.head_dim);
     const size_t rings = (size_t)kMmaWarps * mma_ring_bytes<HD>();
     const size_t smem = states > rings ? states : rings;
-    void (*kern)(AttnArgs) = same_type ? k_attend_mma<T, HD, 1, 2> : k_attend_mma<T, HD, bf16 ? 3 : 2, bf16 ? 3 : 2>;
+    void (*kern)(AttnArgs) = same_type ? k_attend_mma<T, HD, W, 1, 2> : k_attend_mma<T, HD, W, bf16 ? 3 : 2, bf16 ? 3 : 2>;
     if (smem > 48 * 1024 && !smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
     return launch_attend(kern, kMmaWarps, smem, a, n_rows, st);
 }
 
-template <int HD>
+template <int HD, int W>
 cudaError_t run_mma_f32(AttnArgs a, int64_t n_rows, cudaStream_t st) {
     a.chunks = (a.group + kMmaHeads - 1) / kMmaHeads;
     const size_t states = sizeof(float) * (kMmaWarps + 1) * kMmaHeads * state_floats(a.head_dim);
     const size_t rings = (size_t)kMmaWarps * MmaF32<HD>::kRingBytes;
     const size_t smem = states > rings ? states : rings;
-    auto kern = k_attend_mma_f32<HD>;
+    auto kern = k_attend_mma_f32<HD, W>;
     if (!smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
     return launch_attend(kern, kMmaWarps, smem, a, n_rows, st);
 }
 
 template <typename TC>
 cudaError_t run_head(const AttnArgs& a, int cache_type, int64_t n_rows, cudaStream_t st) {
+    // Heads of up to 96 elements in rings made for 128: 100 rows of 2000 keys, 32
+    // heads over 8 of 80, f32, 245 us (276 as 128); 3000 keys, f16, 137 (154).
     if constexpr (sizeof(TC) == 2) {
+        const bool same = a.q_type == cache_type;
         if (use_mma(cache_type, a.group, a.head_dim))
-            return a.head_dim <= 64 ? run_mma<TC, 64>(a, n_rows, a.q_type == cache_type, st)
-                                    : run_mma<TC, 128>(a, n_rows, a.q_type == cache_type, st);
+            return a.head_dim <= 64   ? run_mma<TC, 64, 64>(a, n_rows, same, st)
+                   : a.head_dim <= 96 ? run_mma<TC, 128, 96>(a, n_rows, same, st)
+                                      : run_mma<TC, 128, 128>(a, n_rows, same, st);
     }
     if constexpr (sizeof(TC) == 4) {
         if (use_mma(cache_type, a.group, a.head_dim))
-            return a.head_dim <= 32   ? run_mma_f32<32>(a, n_rows, st)
-                   : a.head_dim <= 64 ? run_mma_f32<64>(a, n_rows, st)
-                                      : run_mma_f32<128>(a, n_rows, st);
+            return a.head_dim <= 32   ? run_mma_f32<32, 32>(a, n_rows, st)
+                   : a.head_dim <= 64 ? run_mma_f32<64, 64>(a, n_rows, st)
+                   : a.head_dim <= 96 ? run_mma_f32<128, 96>(a, n_rows, st)
+                                      : run_mma_f32<128, 128>(a, n_rows, st);
     }
     const int vecs = (a.head_dim + Vec<TC>::n - 1) / Vec<TC>::n;
     if (vecs <= 4) return run_fma<TC, 4, 1>(a, n_rows, st);
