@@ -350,6 +350,25 @@ def test_attention_f32_caches_of_any_magnitude(ops, H, Hk, hd, qt, kpow, vpow):
     check_attention(ops.paged_decode_attention(*a), attention_ref(*a))
 
 
+@pytest.mark.parametrize("ct,H,Hk,hd", [(F32, 4, 1, 32), (F32, 6, 2, 64), (F32, 3, 1, 80), (F32, 9, 1, 128), (BF16, 4, 1, 80)])
+def test_attention_infinite_keys_and_bad_pages_of_grouped_heads(ops, ct, H, Hk, hd):
+    """Keys of -inf under a positive query, and pages outside the cache, in one row: both weigh nothing."""
+    q, ck, cv, table, n = make([200, 47, 16], H, Hk, hd, 16, BF16 if ct == BF16 else F32, ct, hd)
+    q.abs_().clamp_(min=0.01)
+    at = torch.arange(200, device="cuda")
+    gone = (at < 3) | (at >= 64) & (at < 96) | (at == 150)
+    ck[table[0].long()[at[gone] // 16], at[gone] % 16] = -math.inf
+    bad = table.clone()
+    bad[0, 2], bad[0, 7], bad[2, 0] = -1, ck.shape[0], 2 ** 31 - 1
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = ops.paged_decode_attention(q, ck, cv, bad, n, err=err)
+    assert err.item() == PAGE_OOB and not out[2].any()
+    left = at[~gone & (at // 16 != 2) & (at // 16 != 7)]
+    k, v = (c[table[0].long()[left // 16], left % 16][None].contiguous() for c in (ck, cv))
+    check_attention(out[:1], attention_ref(q[:1], k, v, ints([[0]]), ints([len(left)])))
+    check_attention(out[1:2], attention_ref(q[1:2], ck, cv, table[1:2], n[1:2]))
+
+
 def test_attention_many_rows_of_one_request(ops):
     """row_reqs: the tokens of a prefill chunk, each row with its own length, and unordered requests."""
     q, ck, cv, table, n = make([50, 20, 33], 4, 2, 64, 16, F32, F16, 7)
