@@ -11,9 +11,13 @@
 // a larger R' turns T into c (T + S (R - R')) and S into c S, c = 2^(R - R').
 // R is a whole number, so that R, every R - R' and the powers are exact: the
 // states of all threads refer to the same logits (log2 e max x, rounded in each
-// thread, would not).  Logits above 1e37 in magnitude would overflow in
-// x log2 e; a row whose largest is one of them (all of it masked by the type's
-// lowest value, say) is summed again with d = x - m.
+// thread, would not).  From 2^22 on, R is off m log2 e by its own rounding, which
+// grows with it until 2^d is 0 or overflows; x log2 e itself overflows near the
+// end of f32.  So a row whose largest logit is above 2^21 in magnitude (all of it
+// masked by one large value, say) is summed again with d = (x - m) log2 e.
+// Beside a smaller maximum such logits weigh nothing, whatever R their thread
+// had: it leaves a state of 0, or a NaN where a sum overflowed, which sums the row
+// again too.
 //
 // Alternatives.  Each thread keeps the largest logit of every segment of its
 // elements.  The threads form 32 groups; the k-th largest of the 32 group
@@ -72,12 +76,12 @@ __device__ __forceinline__ unsigned long long max_key(unsigned long long a, unsi
 }
 
 // The reference for a maximum m (any m, NaN aside): m log2 e to the nearest
-// whole number, by the shift of 1.5 * 2^23 (beyond 2^22 it stays near m log2 e,
-// where every float is whole).
-constexpr float kHuge = 1e37f;
+// whole number, by the shift of 1.5 * 2^23, for |m| up to kWholeTo; beyond, any
+// finite number near m log2 e.
+constexpr float kWholeTo = 2097152.0f;  // 2^21: m log2 e is below 2^22
 __device__ __forceinline__ float reference_of(float m) {
-    constexpr float kShift = 12582912.0f;
-    const float v = fminf(fmaxf(m, -kHuge), kHuge) * kLog2e;
+    constexpr float kShift = 12582912.0f, kMost = 1e37f;  // kMost log2 e is finite
+    const float v = fminf(fmaxf(m, -kMost), kMost) * kLog2e;
     return __fsub_rn(__fadd_rn(v, kShift), kShift);
 }
 
@@ -136,11 +140,11 @@ struct Row {
     }
 };
 
-// The least maximum whose row the sums above are right for: far enough above
+// The least maximum whose row the sums above are right for.  f16: far enough above
 // what widen() raises -inf to that this weighs nothing.
 template <typename T>
 __device__ __forceinline__ float least_max() {
-    return sizeof(T) == 4 ? -kHuge : __is_same(T, __half) ? -65000.0f : -1e29f;
+    return __is_same(T, __half) ? -65000.0f : -kWholeTo;
 }
 
 // Elements of a vector as f32.  With BOUNDED, 16-bit ones are raised to -1e30
@@ -282,7 +286,7 @@ __device__ __noinline__ void top_by_rounds(Row<T> row, int top_k, int32_t* ids, 
     }
 }
 
-// S and T with d = x - m, in base 2 units, for the rows whose x log2 e may overflow.
+// S and T with d = (x - m) log2 e, for the rows that have no whole reference.
 template <typename T, int NT>
 __device__ __noinline__ void sums_from_differences(Row<T> row, int tid, float m,
                                                    typename Team<NT>::Shared& sh, float* s_out, float* t_out) {
@@ -482,7 +486,7 @@ k_token_logprobs(LogprobArgs a) {
             }
         }
         bool bad = false, huge = false;
-        if (!(m >= least_max<T>() && m <= kHuge && s <= 3e38f)) {  // rare: no distribution, or logits near the type's limits
+        if (!(m >= least_max<T>() && m <= kWholeTo && s <= 3e38f && t == t)) {  // rare: no distribution, or very large logits
             huge = true;
             sums_from_differences<T, NT>(row, tid, m, sh, &s, &t);
             bad = fabsf(m) == INFINITY || s != s;

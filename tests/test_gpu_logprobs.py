@@ -191,3 +191,39 @@ def test_logprobs_twice_the_same_and_replayed(ops):
     g.replay()
     torch.cuda.synchronize()
     check(third, x, tokens, 8)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V", [3, 50, 1000, 6563])
+def test_logprobs_of_any_magnitude(ops, t, V):
+    """Rows of one value from 10^3 to the type's largest power of ten, both signs; rows of a few neighbours of
+    that value; and finite masks of that size around logits of ordinary size."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    last = 4 if t == torch.float16 else 37
+    size = 10.0 ** torch.arange(3, last + 1, device="cuda", dtype=torch.float64).repeat_interleave(2)
+    size = size * torch.tensor([1.0, -1.0], device="cuda").repeat(len(size) // 2)
+    far = size[:, None].expand(-1, V)
+    # the neighbours: up to 8 steps of the type above the value
+    step = torch.finfo(t).eps * size.abs()[:, None]
+    near = far + step * torch.randint(0, 9, far.shape, generator=g, device="cuda")
+    masked = torch.where(torch.rand(far.shape, generator=g, device="cuda") < 0.7, -far.abs(), torch.randn(far.shape, generator=g, device="cuda").double())
+    x = torch.cat([far, near, masked]).to(t)
+    tokens = torch.randint(0, V, (len(x),), generator=g, device="cuda", dtype=torch.int32)
+    k = min(V, 4)
+    check(ops.token_logprobs(x, tokens, top_k=k), x, tokens, k)
+    check(ops.token_logprobs(x, tokens), x, tokens, 0)
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [300, 6563])
+def test_logprobs_beside_large_finite_masks(ops, t, V):
+    """Logits of ordinary size in the last places of a row whose rest is one large value: whole threads see
+    nothing but the mask.  (x log2 e of the odd ones is 122 to 126 above its rounded value.)"""
+    masks = [-2785017856.0, -3998240768.0, -1e12, -1e30, -65504.0, torch.finfo(t).min]
+    x = torch.tensor(masks, device="cuda")[:, None].repeat(1, V)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x[:, -40:] = torch.randn(len(masks), 40, generator=g, device="cuda")
+    x = x.to(t)
+    tokens = torch.tensor([V - 1, V - 7, 0, V - 40, 5, V - 2], device="cuda", dtype=torch.int32)
+    for k in (0, 5):
+        check(ops.token_logprobs(x, tokens, top_k=k), x, tokens, k)
