@@ -527,6 +527,31 @@ __device__ __forceinline__ void terms_of(float x, float y, uint32_t (&t)[N]) {
     }
 }
 
+// P as the products take it: terms of p, of p times kScale for f16, whose second
+// term is times kSecond more.
+template <typename T, int N>
+struct Terms {
+    static constexpr bool f16 = __is_same(T, __half);
+    static_assert(!f16 || N == 2, "P in f16 is two terms");
+    static constexpr float kScale = f16 ? 32768.0f : 1.0f, kSecond = f16 ? 4096.0f : 1.0f;
+    static __device__ __forceinline__ void of(float x, float y, uint32_t (&t)[N]) {
+        if constexpr (f16) {
+            const float f[2] = {x * kScale, y * kScale};
+            t[0] = pack32(f, T{});
+            float r[2];
+            unpack32(t[0], r, T{});
+            const float s[2] = {(f[0] - r[0]) * kSecond, (f[1] - r[1]) * kSecond};
+            t[1] = pack32(s, T{});
+        } else {
+            terms_of<T, N>(x, y, t);
+        }
+    }
+    // The value that the sums of the first (and third) and of the second terms stand for.
+    static __device__ __forceinline__ float sum(float first, float second) {
+        return (first + second * (1.0f / kSecond)) * (1.0f / kScale);
+    }
+};
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
@@ -554,7 +579,10 @@ __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tile
 //   QT terms of q: 1 where q has the cache's type; otherwise 3 of bf16 (24 bits)
 //     or 2 of f16 (22 bits; q is brought to [2^10, 2^11) by a power of two, so
 //     that the second term of all but tiny elements is a normal number).
-//   PT terms of p: 2 for a 16-bit result (16 or 22 bits), 3 of bf16 for f32.
+//   PT terms of p: 2 for a 16-bit result (16 or 22 bits), 3 of bf16 for f32.  f16
+//     holds p times 2^15 and the second term times 2^12 more, as p is at most 1 and
+//     f16 has no exponents below 2^-24: 22 bits down to p = 2^-29, 2^-51 of the row's
+//     largest below.  Unscaled, probabilities below 2^-25 would be lost.
 // A third term is a second product on the same accumulators.
 // Each warp streams its own tiles through a ring in shared memory (cp.async, 16
 // bytes a lane, consecutive lanes on consecutive bytes of a key's row), so no
@@ -718,7 +746,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
             const float p0 = s[2 * n] == -INFINITY ? 0.0f : ex2_approx(s[2 * n] - m);
             const float p1 = s[2 * n + 1] == -INFINITY ? 0.0f : ex2_approx(s[2 * n + 1] - m);
             l += p0 + p1;
-            terms_of<T, PT>(p0, p1, pf[n]);
+            Terms<T, PT>::of(p0, p1, pf[n]);
         }
 #pragma unroll
         for (int j = 0; j < VECS; j += 2) {
@@ -747,7 +775,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int e = 8 * j + 2 * t + k;
-            if (e < hd) st[kStateHead + e] = o[j][k] + o[j][k + 2];
+            if (e < hd) st[kStateHead + e] = Terms<T, PT>::sum(o[j][k], o[j][k + 2]);
         }
     finish<kMmaWarps, kMmaHeads>(a, w, smem);
 }

@@ -505,3 +505,28 @@ def test_a_step_replayed_from_a_graph_and_on_another_stream(ops):
         q = s["qkv"][:, :Hk * hd].view(B, Hk, hd)
         check_attention(s["out"], attention_ref(q, s["ck"], s["cv"], s["table"], n))
     del runs
+
+
+@pytest.mark.parametrize("qt,ct", [(F16, F16), (F32, F16), (BF16, F16), (F32, BF16), (BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("H,Hk,hd", [(4, 4, 64), (4, 2, 64), (16, 2, 32), (12, 4, 80), (8, 1, 128)])
+@pytest.mark.parametrize("nats", [12, 14, 16, 18, 24])
+def test_attention_of_a_key_that_takes_the_weight_and_holds_nothing(ops, qt, ct, H, Hk, hd, nats):
+    """One key whose value is zero, all others `nats` below it: the result is what the others' small
+    probabilities sum to.  The bound is relative to them, as the formula in f32 is."""
+    lens = [2049, 40, 20000]
+    _, ck, cv, table, n = make(lens, H, Hk, hd, 16, qt, ct, hd + nats)
+    g = torch.Generator(device="cuda").manual_seed(nats)
+    q = torch.ones(3, H, hd, device="cuda", dtype=qt)
+    for b, m in enumerate(lens):
+        at = torch.arange(m, device="cuda")
+        pg = table[b].long()[at // 16]
+        # scores are sqrt(hd) times these: the sink's 0
+        low = -nats / hd ** 0.5 + 0.02 * torch.randn(m, Hk, 1, generator=g, device="cuda")
+        low[m // 3] = 0.0
+        ck[pg, at % 16] = low.expand(m, Hk, hd).to(ct)
+        v = 500.0 + 1000.0 * torch.rand(m, Hk, hd, generator=g, device="cuda")
+        v[m // 3] = 0.0
+        cv[pg, at % 16] = v.to(ct)
+    a = (q, ck, cv, table, n)
+    out, lse = ops.paged_decode_attention(*a, return_lse=True)
+    check_attention(out, attention_ref(*a), lse)
