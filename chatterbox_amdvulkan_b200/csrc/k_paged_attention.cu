@@ -570,6 +570,10 @@ template <int HD>
 __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tiles
     return kMmaStages * 2 * kMmaTile * HD * 2;
 }
+// CTAs per SM, by registers (f32 queries take 3 terms on bf16 caches) and shared memory.
+__host__ __device__ constexpr int mma_per_sm(int head_dim, bool f16) {
+    return head_dim > 64 ? 2 : f16 ? 4 : 3;
+}
 
 // S = Q K^T and O = P V by m16n8k16 products, for heads of up to W elements; the
 // rows of the rings are HD elements long.  Rows 0-7 of the first operand
@@ -594,7 +598,7 @@ __host__ __device__ constexpr int mma_ring_bytes() {  // of a warp: K and V tile
 // with 4 heads a CTA took 107 us there.  The 16-byte vectors of a row are permuted by the
 // row's number, which keeps ldmatrix free of bank conflicts.
 template <typename T, int HD, int W, int QT, int PT>
-__global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
+__global__ void __launch_bounds__(kMmaWarps * 32, mma_per_sm(HD, __is_same(T, __half))) k_attend_mma(AttnArgs a) {
     constexpr int KS = W / 16;    // products over the head
     constexpr int VECS = W / 8;   // 16-byte vectors of a row
     constexpr int step = kMmaTile * kMmaWarps;
@@ -754,8 +758,16 @@ __global__ void __launch_bounds__(kMmaWarps * 32) k_attend_mma(AttnArgs a) {
             ldmatrix4_trans(b, vt + (lane & 15) * (HD * 2) + (((j + (lane >> 4)) ^ (lane & 7)) << 4));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                mma16816(o[j + h], pf[0][0], pf[0][1], pf[1][0], pf[1][1], b[2 * h], b[2 * h + 1], T{});
-                if constexpr (PT > 2) mma16816(o[j + h], pf[0][2], 0u, pf[1][2], 0u, b[2 * h], b[2 * h + 1], T{});
+                // The products truncate what they add up: the first terms' sums start
+                // anew each tile and are added with rounding (-3 to 6 % of the time; one
+                // CTA over 65,536 keys: off by less than 1e-5, not 1.1e-4).
+                float d[4] = {0.0f, 0.0f, o[j + h][2], o[j + h][3]};
+                mma16816(d, pf[0][0], pf[0][1], pf[1][0], pf[1][1], b[2 * h], b[2 * h + 1], T{});
+                if constexpr (PT > 2) mma16816(d, pf[0][2], 0u, pf[1][2], 0u, b[2 * h], b[2 * h + 1], T{});
+                o[j + h][0] += d[0];
+                o[j + h][1] += d[1];
+                o[j + h][2] = d[2];
+                o[j + h][3] = d[3];
             }
         }
     }
@@ -1132,9 +1144,9 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
     if (mma && f32) {
         step = head_dim <= 32 ? MmaF32<32>::kStep : head_dim <= 64 ? MmaF32<64>::kStep : MmaF32<128>::kStep;
         per_sm = head_dim <= 32 ? MmaF32<32>::kPerSM : head_dim <= 64 ? MmaF32<64>::kPerSM : MmaF32<128>::kPerSM;
-    } else if (mma) {  // f32 queries take 3 terms, and so more registers, on bf16 caches only
+    } else if (mma) {
         step = kMmaTile * kMmaWarps;
-        per_sm = head_dim > 64 ? 2 : cache_type == CBX_TYPE_F16 ? 4 : 3;
+        per_sm = mma_per_sm((int)head_dim, cache_type == CBX_TYPE_F16);
     } else {
         step = group > 2 ? kRingStep : 8 * (vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
         per_sm = 2;

@@ -530,3 +530,50 @@ def test_attention_of_a_key_that_takes_the_weight_and_holds_nothing(ops, qt, ct,
     a = (q, ck, cv, table, n)
     out, lse = ops.paged_decode_attention(*a, return_lse=True)
     check_attention(out, attention_ref(*a), lse)
+
+
+@pytest.mark.parametrize("ct,H", [(F16, 2), (BF16, 2), (F16, 8), (BF16, 8), (F32, 2), (F32, 8)])
+def test_attention_long_sums_do_not_drift(ops, ct, H):
+    """65,536 keys in one CTA (so many rows that the keys are not split), equal scores, values of one sign:
+    the mean of the values.  The weights are 1 and their sum exact.  A warp has 16,384 keys and adds tiles of
+    8 or more: at most N = 2048 f32 additions, each relative to a partial sum.  Rounded to nearest, their
+    errors are independent of sign with a variance of at most u^2 / 3 (u = 2^-24), together
+    u sqrt(sum (i / N)^2 / 3) = u sqrt(N / 9) = 15 u; six of them: 91 u.  Within a tile at most 17 terms lose
+    2^-23 of the largest, 1, against a sum of 8 * 0.5 or more: 9 u; joins and the quotient 10 u.  Additions
+    that truncate would be off by N / 4 2^-23 = 1024 u."""
+    n, S, hd, R = 65536, 64, 64, 5000
+    g = torch.Generator(device="cuda").manual_seed(H)
+    ck = torch.randn(1, 1, 1, hd, generator=g, device="cuda").to(ct).expand(n // S, S, 1, hd).contiguous()
+    cv = (0.5 + 0.5 * torch.rand(n // S, S, 1, hd, generator=g, device="cuda")).to(ct)
+    table = torch.randperm(n // S, generator=g, device="cuda").to(torch.int32)[None]
+    q = torch.randn(R, H, hd, generator=g, device="cuda")
+    lens = torch.zeros(R, dtype=torch.int32, device="cuda")
+    lens[17] = n
+    assert ops.paged_decode_attention_workspace(R, H, 1, hd, n // S, S, ct) == 0
+    out = ops.paged_decode_attention(q, ck, cv, table, lens, row_reqs=torch.zeros_like(lens))
+    want = cv.double().mean((0, 1, 2))
+    off = (out[17].double() / want - 1).abs().max().item() * 2.0 ** 24
+    assert off < 91 + 9 + 10, off
+    assert not out[:17].any() and not out[18:].any()
+
+
+@pytest.mark.parametrize("ct,H", [(F16, 2), (BF16, 2), (F16, 8), (BF16, 8), (F32, 2), (F32, 8)])
+def test_attention_long_weighted_sums_do_not_drift(ops, ct, H):
+    """The same with weights of all sizes around 1 (scores with a deviation of a half), which the values'
+    few bits do not make exact: 91 u for the sums as above; the sum of the weights, 2048 additions a lane,
+    the same averaged over the 4 lanes: 46 u; a tile's sum is a quarter of 16 times its largest term or more:
+    20 u; e^ 8 u; the terms of q 4 u (the scores' own errors have either sign and average out); joins and the
+    quotient 10 u."""
+    n, S, hd, R = 65536, 64, 64, 5000
+    g = torch.Generator(device="cuda").manual_seed(H)
+    ck = (0.5 * torch.randn(n // S, S, 1, hd, generator=g, device="cuda")).to(ct)
+    cv = (0.5 + 0.5 * torch.rand(n // S, S, 1, hd, generator=g, device="cuda")).to(ct)
+    table = torch.randperm(n // S, generator=g, device="cuda").to(torch.int32)[None]
+    q = torch.randn(R, H, hd, generator=g, device="cuda")
+    lens = torch.zeros(R, dtype=torch.int32, device="cuda")
+    lens[17] = n
+    out = ops.paged_decode_attention(q, ck, cv, table, lens, row_reqs=torch.zeros_like(lens))
+    k, v = (c[table[0].long()].flatten(0, 2).double() for c in (ck, cv))
+    want = torch.softmax(q[17].double() @ k.T / hd ** 0.5, -1) @ v
+    off = (out[17].double() / want - 1).abs().max().item() * 2.0 ** 24
+    assert off < 91 + 46 + 20 + 8 + 4 + 10, off
