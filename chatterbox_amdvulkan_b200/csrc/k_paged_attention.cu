@@ -229,6 +229,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t p) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t lds32(uint32_t p) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(p) : "memory");
+    return v;
+}
 __device__ __forceinline__ float lds_f32(uint32_t p) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
@@ -727,13 +732,36 @@ __global__ void __launch_bounds__(kMmaWarps * 32, mma_per_sm(HD, __is_same(T, __
             }
         }
         float best = m;
+        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool in = keys >> (2 * t + (i & 1) + (i >> 1) * 8) & 1;
             s[i] = in ? s[i] * scale : -INFINITY;
             best = fmaxf(best, s[i]);
+            if (QT > 1) odd |= s[i] != s[i];
         }
-        if (__any_sync(0xffffffffu, best > m)) {
+        if (__any_sync(0xffffffffu, best > m || odd)) {
+            // An infinite key times a term of q that is 0 is a NaN, and so is the sum with
+            // one of the other sign: such a tile is scored again by f32 FMAs.
+            if (QT > 1 && __any_sync(0xffffffffu, odd)) {
+                with_type(a.q, a.q_type, [&](auto* p) {
+                    p += (int64_t)w.row * a.q_stride + (int64_t)(w.head0 + g) * hd;
+                    for (int n = 0; n < 4; ++n) {
+                        const int r = (n >> 1) * 8 + 2 * t + (n & 1);
+                        float sum = 0.0f;
+                        for (int i = 0; i < hd && g < w.heads; i += 2) {
+                            float k[2];
+                            unpack32(lds32(kt + r * (HD * 2) + (((i >> 3) ^ (r & 7)) << 4) + (i & 7) * 2), k, T{});
+                            sum = fmaf(to_f(p[i + 1]), k[1], fmaf(to_f(p[i]), k[0], sum));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k == n) s[k] = keys >> r & 1 ? sum * a.scale_log2 : -INFINITY;
+                    }
+                });
+#pragma unroll
+                for (int i = 0; i < 4; ++i) best = fmaxf(best, s[i]);
+            }
             best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
             best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
             const float c = rescale(m, best);

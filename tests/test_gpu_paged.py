@@ -577,3 +577,9 @@ def test_attention_long_weighted_sums_do_not_drift(ops, ct, H):
     want = torch.softmax(q[17].double() @ k.T / hd ** 0.5, -1) @ v
     off = (out[17].double() / want - 1).abs().max().item() * 2.0 ** 24
     assert off < 91 + 46 + 20 + 8 + 4 + 10, off
+
+
+@pytest.mark.parametrize("qt,ct,H,Hk", [(F32, F16, 8, 2), (F32, BF16, 8, 1), (BF16, F16, 4, 2), (F16, BF16, 2, 1), (F16, F32, 3, 1)])
+def test_attention_scores_of_minus_infinity_with_q_of_another_type(ops, qt, ct, H, Hk):
+    """The same where the tensor cores take q in several terms, some of them 0."""
+    test_attention_scores_of_minus_infinity(ops, qt, ct, H, Hk)
