@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 from typing import NamedTuple
 
 import numpy as np
@@ -603,10 +604,13 @@ _I32, _F32 = torch.int32, torch.float32
 
 
 def _on_device(fn):
-    """``_on_tensor_device`` in fewer operations: run with the first tensor's device current."""
+    """``_on_tensor_device`` in fewer operations: run with the device of the first parameter's tensor
+    current, whichever place its keyword has.  The wrappers compare the other tensors with it."""
+    first = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
     def wrapper(*args, **kw):
-        t = args[0] if args else next(iter(kw.values()), None)
+        t = args[0] if args else kw.get(first)
         dev = t.get_device() if isinstance(t, torch.Tensor) else -1
         if dev >= 0 and dev != _current_device():
             with torch.cuda.device(dev):

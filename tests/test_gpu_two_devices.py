@@ -103,3 +103,24 @@ def test_batched_gathers_alternate_between_devices(ops):
             seq = ops.t3_embed_sequence_batched(_on(dev, tok), _on(dev, ids), _on(dev, pos), 3,
                                                 cond=_on(dev, cond))
             assert np.array_equal(seq.cpu().numpy(), np.stack(seq_ref))
+
+
+def test_paged_operators_follow_their_tensors_device(ops):
+    """The paged wrappers with the tensors on cuda:1 while cuda:0 is current, arguments in any order."""
+    torch.cuda.set_device(0)
+    for dev in (1, 0, 1):
+        d = torch.device("cuda", dev)
+        i32 = dict(dtype=torch.int32, device=d)
+        p = ops.paged_plan(page_size=4, n_new=torch.tensor([5, 1], **i32), max_rows=6, free_list=torch.arange(8, **i32),
+                           n_free=torch.tensor([8], **i32), block_table=torch.full((2, 4), -1, **i32),
+                           n_blocks=torch.zeros(2, **i32), seq_lens=torch.tensor([5, 1], **i32))
+        ck, cv = (torch.zeros(8, 4, 1, 32, device=d) for _ in range(2))
+        qkv = torch.randn(6, 96, device=d)
+        q, _ = ops.qkv_kv_append_paged(bias=None, slots=p.slots, cache_k=ck, cache_v=cv, qkv=qkv)
+        out = ops.paged_decode_attention(scale=0.5, cache_k=ck, cache_v=cv, block_table=p.block_table,
+                                         seq_lens=p.row_lens, row_reqs=p.row_reqs, q=q.view(6, 1, 32))
+        lp = ops.token_logprobs(tokens=None, top_k=2, logits=out.view(6, 32))
+        assert out.device == d and torch.cuda.current_device() == 0 and p.err.item() == 0
+        s = (0.5 * qkv[:5, :32].double() @ qkv[:5, 32:64].double().T).masked_fill(torch.ones(5, 5, device=d).triu(1) > 0, -torch.inf)
+        assert (out[:5, 0] - torch.softmax(s, -1) @ qkv[:5, 64:].double()).abs().max() < 1e-5
+        assert torch.equal(out[5, 0], qkv[5, 64:]) and torch.equal(lp.top_ids.long(), out.view(6, 32).topk(2).indices)

@@ -190,3 +190,62 @@ def test_definitions_agree_with_torch():
     y = torch.log_softmax(x, -1)
     assert torch.allclose(lp, y[[0, 1, 2], [1, 2, 3]]) and torch.allclose(ent, torch.distributions.Categorical(logits=x).entropy())
     assert torch.allclose(top, y.topk(4).values)
+
+
+class OnDevice1(torch.Tensor):
+    """A host tensor that says it is on CUDA device 1."""
+    def get_device(self):
+        return 1
+
+
+def test_wrappers_run_with_their_tensors_device_current(monkeypatch):
+    """Tensors on device 1 while device 0 is current, the arguments in any order of keywords: every call
+    reaches the library with device 1 current, or is refused."""
+    from chatterbox_amdvulkan_b200 import ops
+    state, calls = {"dev": 0}, []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, state["dev"] = state["dev"], self.dev
+
+        def __exit__(self, *a):
+            state["dev"] = self.before
+
+    monkeypatch.setattr(ops, "_current_device", lambda: state["dev"])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: None)
+    monkeypatch.setattr(ops, "_workspace_bytes", lambda *a: 0)
+    monkeypatch.setattr(ops, "_fn", lambda name: lambda *a: calls.append((name, state["dev"])) or 0)
+
+    def on1(t):
+        return t.as_subclass(OnDevice1)
+
+    def z(*s):
+        return on1(torch.zeros(*s, dtype=torch.int32))
+
+    k = on1(torch.zeros(5, 16, 2, 32))
+    err = z(1)
+    plan = dict(page_size=16, err=err, n_new=None, max_rows=3, free_list=z(20), n_free=z(1), block_table=z(3, 4),
+                n_blocks=z(3), out=[z(n) for n in (3, 3, 3, 3, 4, 12, 3, 20, 1)], seq_lens=z(3))
+    append = dict(bias=None, with_q=True, err=err, slots=z(3), cache_k=k, cache_v=k, qkv=on1(torch.zeros(3, 256)))
+    attend = dict(scale=1.0, row_reqs=None, err=err, seq_lens=z(3), block_table=z(3, 4), cache_k=k, cache_v=k,
+                  q=on1(torch.zeros(3, 4, 32)))
+    score = dict(top_k=2, tokens=None, err=err, logits=on1(torch.zeros(3, 40)))
+    for fn, kw in ((ops.paged_plan, plan), (ops.qkv_kv_append_paged, append), (ops.paged_decode_attention, attend),
+                   (ops.token_logprobs, score)):
+        fn(**kw)
+        fn(**dict(reversed(kw.items())))
+        first, *rest = reversed(kw.items())
+        fn(first[1], **dict(rest))
+    assert len(calls) == 12 and all(dev == 1 for _, dev in calls) and state["dev"] == 0
+    # one tensor on the host, or on another device, is refused
+    other = torch.zeros(3, dtype=torch.int32)
+    for fn, kw in ((ops.paged_plan, {**plan, "n_blocks": other}), (ops.qkv_kv_append_paged, {**append, "slots": other}),
+                   (ops.paged_decode_attention, {**attend, "seq_lens": other}),
+                   (ops.token_logprobs, {**score, "tokens": other})):
+        with pytest.raises(ValueError):
+            fn(**kw)
+    assert len(calls) == 12
