@@ -23,9 +23,9 @@
 //    pages, then the cluster barrier makes them visible and ends all reads of
 //    what is overwritten.
 // Measured: 512 requests of 513 blocks, 262,656 pages, one token each: 5.1 us
-// with new outputs (20.3 us with the cluster), 7.0 us in place; 64 requests,
-// 65,536 rows: 4.1 us (11.7) and 10.6 us; 64 requests, one token each, in place:
-// 4.1 us.  (Four rows to a thread, with 16-byte stores, was slower: 8.2 and 6.5
+// with new outputs (20.3 us with the cluster), 8.2 us in place (1.0 of it the check
+// of the pages that stay); 64 requests, 65,536 rows: 4.1 us (11.7) and 11.1 us; 64
+// requests, one token each, in place: 4.8 us.  (Four rows to a thread, with 16-byte stores, was slower: 8.2 and 6.5
 // us with new outputs.)
 #include "cbx_common.cuh"
 
@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a) {
         return i < n_free ? a.free_in[i] : released(i - n_free);
     };
 
-    // Tables and counts.  In place the kept entries stay; those behind the last
-    // page become -1 whatever they held.
+    // Tables and counts.  In place the kept entries stay, but are checked like the
+    // others; those behind the last page become -1 whatever they held.
     auto write_entry = [&](int b, int j, int need, int have) {
         const int64_t i = (int64_t)b * a.max_blocks + j;
         const int left = top - s_pop[b];  // pages on the stack when b's turn comes
@@ -228,8 +228,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(PlanArgs a) {
         const int lane = tid & 31, warps = (int)(all / 32);
         for (int b = (int)(me / 32); b < B; b += warps) {
             const int need = s_need[b], have = s_have[b];
-            for (int j = (a.table == a.table_in ? min(need, have) : 0) + lane; j < a.max_blocks; j += 32)
-                write_entry(b, j, need, have);
+            int first = 0;
+            if (a.table == a.table_in) {  // (checked before the barrier: 10.1, not 8.2 us for the 512 requests)
+                first = min(need, have);
+                const int32_t* kept = a.table_in + (int64_t)b * a.max_blocks;
+#pragma unroll 4
+                for (int j = lane; j < first; j += 32)
+                    if (kept[j] < 0 || kept[j] >= a.n_pages) flags |= CBX_EFLAG_PAGE_OOB;
+            }
+            for (int j = first + lane; j < a.max_blocks; j += 32) write_entry(b, j, need, have);
         }
     } else {
         const int64_t entries = (int64_t)B * a.max_blocks;

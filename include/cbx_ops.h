@@ -447,7 +447,9 @@ CBX_API int cbx_qkv_kv_append(const float* qkv, int64_t qkv_row_stride, const fl
  * slot -1); a negative length, n_new outside [0, seq_lens], a length above
  * max_blocks * page_size, more rows than max_rows, state counts outside their
  * range (CBX_EFLAG_LENGTH: clamped, rows behind max_rows dropped); a page id
- * outside [0, n_pages) (CBX_EFLAG_PAGE_OOB, slot -1).
+ * outside [0, n_pages) in a block that a request keeps or is given
+ * (CBX_EFLAG_PAGE_OOB, slot -1; pages that go back on the stack are not looked
+ * at until they are given out again).
  * n_reqs <= CBX_PAGED_MAX_REQS; n_pages * page_size, n_reqs * max_blocks and
  * max_rows below 2^31.  Integer results, the same in every run.
  * ------------------------------------------------------------------------- */

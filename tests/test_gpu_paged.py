@@ -583,3 +583,17 @@ def test_attention_long_weighted_sums_do_not_drift(ops, ct, H):
 def test_attention_scores_of_minus_infinity_with_q_of_another_type(ops, qt, ct, H, Hk):
     """The same where the tensor cores take q in several terms, some of them 0."""
     test_attention_scores_of_minus_infinity(ops, qt, ct, H, Hk)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("table", [[[7, 1, 2, -1], [-3, 4, 5, -1], [6, 3, 0, -1]], [[7, 1, 2, -1], [8, 4, 99, -1], [6, 3, 0, -1]],
+                                   [[2 ** 31 - 1, 1, 2, -1], [8, 4, 9, -1], [6, 3, 0, -1]]])
+def test_plan_flags_bad_pages_that_a_request_keeps(ops, in_place, table):
+    """A page outside the pool in a block that none of the step's rows lies in: flagged, in place or not."""
+    lens, new, have = [9, 12, 0], [1, 0, 0], [3, 3, 0]
+    free = [10, 11, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0]
+    ref = plan_ref(lens, new, table, have, free, 2, 4, 4)
+    assert ref[9] == PAGE_OOB
+    p = ops.paged_plan(ints(lens), ints(table), ints(have), ints(free), ints([2]), 4, n_new=ints(new), max_rows=4,
+                       in_place=in_place)
+    check_plan(p, ref)
