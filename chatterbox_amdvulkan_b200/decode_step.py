@@ -176,8 +176,8 @@ class T3BatchedDecode:
 
 class PagedCacheFull(RuntimeError):
     """A request's tokens found no page (the pool is empty, or its row of the
-    block table full) or its length was out of range: its new K / V rows were
-    not written and the step's output for it is invalid."""
+    block table full) or its length was out of range: its new K / V rows are
+    missing or mean nothing, and the step's output for it is invalid."""
 
 
 class T3PagedDecode:
@@ -270,11 +270,12 @@ class T3PagedDecode:
 
     def check_errors(self) -> None:
         """Read and clear the device error word (synchronises with the stream)."""
-        from ._lib import EFLAG_LENGTH, EFLAG_NO_PAGE
+        from ._lib import EFLAG_LENGTH, EFLAG_NO_PAGE, EFLAG_POS_OOB
         flags = int(self.err.item())
         if flags:
             self.err.zero_()
-            if flags & (EFLAG_NO_PAGE | EFLAG_LENGTH):
+            # a length between max_context and the end of its last page has a page, but no position
+            if flags & (EFLAG_NO_PAGE | EFLAG_LENGTH | EFLAG_POS_OOB):
                 raise PagedCacheFull(
                     "a request found no page for its new tokens, or its length is outside "
                     f"[0, {self.ctx}] (device error flags 0x{flags:x})")

@@ -128,3 +128,21 @@ def test_an_exhausted_pool_is_reported_and_the_next_step_runs(dec):
     m.step(ints([1] * 12), ints([4, 0, 6]), ints([0, 0, 6]))  # the first one cut back to its first page
     with pytest.raises(dec.PagedCacheFull):
         m.step(ints([1] * 3), ints([17, 0, 0]), ints([1, 0, 0]))
+
+
+def test_a_length_between_the_context_and_its_last_page_is_reported(dec):
+    """max_context 10 in pages of 4: lengths 11 and 12 have a page, but no position."""
+    m = dec.T3PagedDecode(1, max_reqs=2, n_pages=6, page_size=4, max_context=10, D=64, H=1, F=64, vocab=50)
+    m.step(ints([1] * 10), ints([10, 0]), ints([10, 0]))
+    for n in (11, 12):
+        with pytest.raises(dec.PagedCacheFull, match="10"):
+            m.step(ints([1] * (n - 10)), ints([n, 0]), ints([n - 10, 0]))
+    h, _ = m.step(ints([2, 3]), ints([10, 1]), ints([1, 1]))
+    assert h.isfinite().all()
+
+
+def test_a_step_without_rows_ends_requests(dec):
+    m = dec.T3PagedDecode(1, max_reqs=2, n_pages=6, page_size=4, max_context=10, D=64, H=1, F=64, vocab=50)
+    m.step(ints([1] * 10), ints([10, 0]), ints([10, 0]))
+    h, lp = m.step(ints([]), ints([0, 0]), ints([0, 0]), top_k=2)
+    assert h.shape == (0, 64) and lp.entropy.numel() == 0 and m.n_free.item() == 6
