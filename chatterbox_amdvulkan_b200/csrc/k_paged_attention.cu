@@ -1140,6 +1140,18 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttnArgs a) {
     if (a.lse && threadIdx.x == 0) a.lse[rh] = lse_of(mm, ll);
 }
 
+// Shared memory of the FMA kernel for G heads.
+template <typename Shape>
+size_t fma_smem(int G, int64_t head_dim) {
+    return sizeof(float) * (Shape::kWarps + 1) * G * state_floats((int)head_dim) + (size_t)Shape::kRingBytes * Shape::kWarps;
+}
+// Whether an SM holds two CTAs of the ring with four heads (heads of more than 128
+// elements; each CTA takes 1 KB of the 228 more).
+bool two_rings(int cache_type, int64_t head_dim) {
+    const size_t smem = cache_type == CBX_TYPE_F32 ? fma_smem<Fma<32, 2, true>>(4, head_dim) : fma_smem<Fma<32, 1, true>>(4, head_dim);
+    return 2 * (smem + 1024) <= 228 * 1024;
+}
+
 // Query heads of a CTA.
 int group_chunk(int group) { return group >= 3 ? 4 : group; }
 bool use_mma(int cache_type, int group, int head_dim) {
@@ -1176,8 +1188,9 @@ Splits choose_splits(int64_t n_rows, int64_t n_kv, int group, int64_t head_dim, 
         step = kMmaTile * kMmaWarps;
         per_sm = mma_per_sm((int)head_dim, cache_type == CBX_TYPE_F16);
     } else {
-        step = group > 2 ? kRingStep : 8 * (vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
-        per_sm = 2;
+        const bool ring = group > 2 && two_rings(cache_type, head_dim);
+        step = ring ? kRingStep : 8 * (vecs <= 8 ? 32 : vecs <= 16 ? 16 : 8);
+        per_sm = group > 2 && !ring ? 1 : 2;  // four heads of 216 and more f32 elements: 253 registers
     }
     const int64_t resident = num_sms() * per_sm;
     const int64_t ctas = n_rows * n_kv * ((group + gc - 1) / gc);
@@ -1212,24 +1225,35 @@ template <typename TC, int VL, int VPL, int G, bool RING>
 cudaError_t run_fma_heads(AttnArgs a, int64_t n_rows, cudaStream_t st) {
     using Shape = Fma<VL, VPL, RING>;
     a.chunks = (a.group + G - 1) / G;
-    const size_t smem = sizeof(float) * (Shape::kWarps + 1) * G * state_floats(a.head_dim) +
-                        (size_t)Shape::kRingBytes * Shape::kWarps;
+    const size_t smem = fma_smem<Shape>(G, a.head_dim);
     auto kern = k_attend_fma<TC, VL, VPL, G, RING>;
     if (smem > 48 * 1024 && !smem_opt_in(kern, smem)) return cudaErrorInvalidValue;
     return launch_attend(kern, Shape::kWarps, smem, a, n_rows, st);
 }
 
-// Heads of more than 128 elements, four at a time, take the ring, others the
-// registers.  Ring / registers / registers with two at a time, in us (B200):
-//   40 rows of 4000 keys, 32 heads over 4 of 160, f32      426 / 477 / 688
-//   94 rows of 2511 keys, 16 heads over 2 of 256, bf16     242 / 348 / 429
-//   30 rows of 2511 keys, 8 heads over 2 of 256, f32       99 / 74 / 108
+// Heads of more than 128 elements, four at a time, take the ring where an SM holds
+// two of its CTAs (f32: up to 208 elements), others the registers.  Ring / registers
+// / registers with two at a time, in us (B200):
+//   40 rows of 4000 keys, 32 heads over 4 of 160, f32      426 / 439 / 688
+//   64 rows of 1000 keys, 16 heads over 4 of 200, f32      85 / 102
+//   30 rows of 2511 keys, 8 heads over 2 of 160, f32       58 / 63
+//   94 rows of 2511 keys, 16 heads over 2 of 256, bf16     242 / 323 / 429
+//   30 rows of 2511 keys, 8 heads over 2 of 256, bf16      67 / 63
+//   300 rows of 500 keys, 12 heads over 4 of 192, bf16     150 / 230
+//   94 rows of 2511 keys, 16 heads over 2 of 256, f32      489 / 328
+//   40 rows of 4000 keys, 32 heads over 4 of 256, f32      667 / 450
+//   12 rows of 9000 keys, 8 heads over 1 of 224, f32       113 / 84
+//   30 rows of 2511 keys, 8 heads over 2 of 256, f32       91 / 67 / 108
 //   128 rows up to 8196 keys, 16 heads of 64, bf16         326 / 296 (1.98 GB: 6.7 TB/s)
 template <typename TC, int VL, int VPL>
 cudaError_t run_fma(const AttnArgs& a, int64_t n_rows, cudaStream_t st) {
     constexpr bool wide = VL * VPL * Vec<TC>::n > 128;  // heads that the tensor-core kernels do not take
-    if constexpr (wide)
-        if (a.group > 2) return run_fma_heads<TC, VL, VPL, 4, true>(a, n_rows, st);
+    if constexpr (wide) {
+        constexpr int type = sizeof(TC) == 4 ? CBX_TYPE_F32 : CBX_TYPE_F16;  // of this size
+        if (a.group > 2 && two_rings(type, a.head_dim)) return run_fma_heads<TC, VL, VPL, 4, true>(a, n_rows, st);
+        if constexpr (sizeof(TC) == 4)
+            if (a.group > 2) return run_fma_heads<TC, VL, VPL, 4, false>(a, n_rows, st);
+    }
     if constexpr (wide || sizeof(TC) == 4)
         if (a.group == 2) return run_fma_heads<TC, VL, VPL, 2, false>(a, n_rows, st);
     return run_fma_heads<TC, VL, VPL, 1, false>(a, n_rows, st);

@@ -597,3 +597,19 @@ def test_plan_flags_bad_pages_that_a_request_keeps(ops, in_place, table):
     p = ops.paged_plan(ints(lens), ints(table), ints(have), ints(free), ints([2]), 4, n_new=ints(new), max_rows=4,
                        in_place=in_place)
     check_plan(p, ref)
+
+
+@pytest.mark.parametrize("qt,ct", [(F32, F32), (BF16, F32), (F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("H,Hk,hd", [(3, 1, 136), (10, 2, 160), (7, 1, 208), (6, 2, 216), (5, 1, 248), (8, 2, 256)])
+@pytest.mark.parametrize("lens", list(LENS))
+def test_attention_grouped_heads_of_more_than_128_elements(ops, qt, ct, H, Hk, hd, lens):
+    """Both kernels for them (f32: up to 208 elements, and above), with chunks of four heads that are not full."""
+    a = make(LENS[lens], H, Hk, hd, 16, qt, ct, hd + H)
+    out, lse = ops.paged_decode_attention(*a, return_lse=True)
+    check_attention(out, attention_ref(*a), lse)
+    if lens == "edge":  # unsplit, rows of all lengths
+        many = torch.randn(300, H, hd, device="cuda").to(qt)
+        reqs = torch.arange(300, device="cuda", dtype=torch.int32) % len(LENS[lens])
+        n = a[4][reqs.long()].contiguous()
+        got = ops.paged_decode_attention(many, *a[1:4], n, row_reqs=reqs)
+        check_attention(got, attention_ref(many, *a[1:4], n, reqs))
