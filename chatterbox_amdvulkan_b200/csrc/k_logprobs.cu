@@ -147,15 +147,23 @@ __device__ __forceinline__ float least_max() {
     return __is_same(T, __half) ? -65000.0f : -kWholeTo;
 }
 
-// Elements of a vector as f32.  With BOUNDED, 16-bit ones are raised to -1e30
-// (bf16) or the lowest finite value (f16), two in one instruction: no weight
-// beside a maximum of least_max or more, but a finite x log2 e.  NaN stays.
+// What widen() raises lower 16-bit logits to: the lowest finite value (f16), -2^100
+// (bf16; its product with log2 e is exact, so its difference from its own
+// reference is 0).
+template <typename T>
+__device__ __forceinline__ float lowest() {
+    return __is_same(T, __half) ? -65504.0f : -0x1p100f;
+}
+
+// Elements of a vector as f32.  With BOUNDED, 16-bit ones are raised to lowest(),
+// two in one instruction: no weight beside a maximum of least_max or more, but a
+// finite x log2 e.  NaN stays.
 template <typename T, bool BOUNDED>
 __device__ __forceinline__ void widen(uint4 w, float2 (&f)[Vec<T>::n / 2]) {
     if constexpr (BOUNDED && sizeof(T) == 2) {
         constexpr bool bf16 = __is_same(T, __nv_bfloat16);
         using T2 = std::conditional_t<bf16, __nv_bfloat162, __half2>;
-        const float low[2] = {bf16 ? -1e30f : -65504.0f, bf16 ? -1e30f : -65504.0f};
+        const float low[2] = {lowest<T>(), lowest<T>()};
         const uint32_t b = pack32(low, T{});
         auto raise = [&](uint32_t v) {
             const T2 r = __hmax2_nan(*reinterpret_cast<const T2*>(&v), *reinterpret_cast<const T2*>(&b));
@@ -380,19 +388,22 @@ k_token_logprobs(LogprobArgs a) {
                 fetch(Row<T>(a, r + stride), 0, ahead);
             }
             const float m = max_of(w, T{});
+            // The largest of the values summed: a thread with nothing but -inf so far must
+            // not take that as its reference, or its sums overflow.
+            const float most = kBounded ? fmaxf(m, lowest<T>()) : m;
             if ((b + 1) * kBatch <= row.nv) {
                 float2 f[kUnroll * EV / 2];
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
                     widen<T, kBounded>(w[u], *reinterpret_cast<float2(*)[EV / 2]>(f + u * EV / 2));
-                add<kUnroll * EV, kBounded>(st, f, m);
+                add<kUnroll * EV, kBounded>(st, f, most);
             } else {
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
                     if (b * kBatch + u * NT < row.nv) {
                         float2 f[EV / 2];
                         widen<T, kBounded>(w[u], f);
-                        add<EV, kBounded>(st, f, m);
+                        add<EV, kBounded>(st, f, most);
                     }
             }
             if (TOP) {

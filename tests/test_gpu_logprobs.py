@@ -227,3 +227,19 @@ def test_logprobs_beside_large_finite_masks(ops, t, V):
     tokens = torch.tensor([V - 1, V - 7, 0, V - 40, 5, V - 2], device="cuda", dtype=torch.int32)
     for k in (0, 5):
         check(ops.token_logprobs(x, tokens, top_k=k), x, tokens, k)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V", [40, 130, 6563, 50276])
+def test_logprobs_of_half_masked_vocabularies(ops, t, V):
+    """-inf over whole threads: the first half, the last half, all but the last place, every block but one."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = 3.0 * torch.randn(4, V, generator=g, device="cuda")
+    x[0, :V // 2] = -math.inf
+    x[1, V // 2:] = -math.inf
+    x[2, :-1] = -math.inf
+    x[3, :V // 3], x[3, V // 3 + 9:] = -math.inf, -math.inf
+    x = torch.cat([x, x - 1000.0]).to(t)
+    tokens = torch.tensor([V - 1, 0, V - 1, V // 3] * 2, dtype=torch.int32, device="cuda")
+    for k in (0, 3):
+        check(ops.token_logprobs(x, tokens, top_k=k), x, tokens, k)
