@@ -28,6 +28,16 @@ int num_sms();
 bool pdl_enabled();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// NULL is aligned to anything.
+inline bool aligned_to(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % (unsigned)size == 0; }
+// Whether [p, p + bytes) meets one of n > 0 rows of `width` bytes, `stride` >= width apart.
+inline bool meets_rows(const void* p, int64_t bytes, const void* rows, int64_t n, int64_t stride, int64_t width) {
+    if (!p || bytes <= 0 || width <= 0) return false;
+    const int64_t a = (int64_t)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(rows));
+    // the first row that ends behind p
+    const int64_t r = a < width ? 0 : (a - width) / stride + 1;
+    return r < n && r * stride < a + bytes;
+}
 inline bool valid_type(int t) { return t == CBX_TYPE_F32 || t == CBX_TYPE_F16 || t == CBX_TYPE_BF16; }
 __host__ __device__ inline int type_size(int t) { return t == CBX_TYPE_F32 ? 4 : 2; }
 

@@ -606,8 +606,10 @@ extern "C" CBX_API int cbx_token_logprobs(const void* logits, int type, int64_t 
     if (!logits || (tokens != nullptr) != (logprob != nullptr) || (tokens && !err_word) ||
         (top_k > 0 && (!top_ids || !top_logprobs)))
         return fail(CBX_ERR_INVALID_ARG, "%s: NULL argument", name);
-    if (reinterpret_cast<uintptr_t>(logits) % (unsigned)type_size(type))
-        return fail(CBX_ERR_INVALID_ARG, "%s: logits are not aligned to their type", name);
+    if (!aligned_to(logits, type_size(type)) || !aligned_to(tokens, 4) || !aligned_to(logprob, 4) ||
+        !aligned_to(entropy, 4) || !aligned_to(top_ids, 4) || !aligned_to(top_logprobs, 4) ||
+        !aligned_to(err_word, 4))
+        return fail(CBX_ERR_INVALID_ARG, "%s: an argument is not aligned to its type", name);
     LogprobArgs a{logits, row_stride, n_rows, (int)vocab, tokens, (int)top_k, logprob, entropy,
                   top_ids, top_logprobs, err_word};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

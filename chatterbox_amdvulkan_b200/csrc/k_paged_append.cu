@@ -196,6 +196,12 @@ extern "C" CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type,
     if (n_rows == 0) return ok();
     if (!qkv || !slots || !cache_k || !cache_v || !err_word)
         return fail(CBX_ERR_INVALID_ARG, "%s: NULL qkv, slots, cache or err_word", name);
+    const int si = type_size(qkv_type), sc = type_size(cache_type);
+    if (!aligned_to(qkv, si) || !aligned_to(q_out, si) || !aligned_to(cache_k, sc) || !aligned_to(cache_v, sc) ||
+        !aligned_to(qkv_bias, 4) || !aligned_to(slots, 4) || !aligned_to(err_word, 4))
+        return fail(CBX_ERR_INVALID_ARG, "%s: an argument is not aligned to its type", name);
+    if (meets_rows(q_out, n_rows * q_dim * si, qkv, n_rows, qkv_row_stride * si, (q_dim + 2 * kv_dim) * si))
+        return fail(CBX_ERR_INVALID_ARG, "%s: q_out overlaps qkv", name);
     PagedAppendArgs a{qkv, qkv_row_stride, qkv_bias, n_rows, (int)q_dim, (int)kv_dim, slots,
                       cache_k, cache_v, page_stride, (int)page_size, (int)(n_pages * page_size),
                       page_stride == page_size * kv_dim, 0, q_out, err_word};

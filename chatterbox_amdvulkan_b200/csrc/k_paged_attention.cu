@@ -1387,6 +1387,13 @@ extern "C" CBX_API int cbx_paged_decode_attention(
     if (n_rows == 0) return ok();
     if (!q || !cache_k || !cache_v || !table || !seq_lens || !out || !err_word)
         return fail(CBX_ERR_INVALID_ARG, "%s: NULL argument", name);
+    const int qs = type_size(q_type);
+    if (!aligned_to(q, qs) || !aligned_to(out, qs) || !aligned_to(table, 4) || !aligned_to(row_reqs, 4) ||
+        !aligned_to(seq_lens, 4) || !aligned_to(lse, 4) || !aligned_to(err_word, 4))
+        return fail(CBX_ERR_INVALID_ARG, "%s: an argument is not aligned to its type", name);
+    if (meets_rows(out, n_rows * n_heads * head_dim * qs, q, n_rows, q_row_stride * qs, n_heads * head_dim * qs) ||
+        meets_rows(lse, n_rows * n_heads * 4, q, n_rows, q_row_stride * qs, n_heads * head_dim * qs))
+        return fail(CBX_ERR_INVALID_ARG, "%s: an output overlaps q", name);
     if (!aligned16(cache_k) || !aligned16(cache_v) ||
         (page_stride * type_size(cache_type)) % 16)
         return fail(CBX_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned", name);

@@ -319,12 +319,15 @@ extern "C" CBX_API int cbx_paged_plan(const int32_t* seq_lens, const int32_t* n_
     {
         // Each state output may be its own input; no other overlap.
         const int64_t nt = n_reqs * max_blocks;
+        bool aligned = aligned_to(err_word, 4);
         const void* in[6] = {table_in, n_blocks_in, free_in, n_free_in, seq_lens, n_new};
         const int64_t ni[6] = {nt, n_reqs, n_pages, 1, n_reqs, n_reqs};
         const void* out[9] = {table_out, n_blocks_out, free_out, n_free_out, slots,
                               positions, row_reqs, row_lens, row_start};
         const int64_t no[9] = {nt, n_reqs, n_pages, 1, max_rows,
                                max_rows, max_rows, max_rows, n_reqs + 1};
+        for (int i = 0; i < 9; ++i) aligned = aligned && aligned_to(out[i], 4) && aligned_to(in[i < 6 ? i : 0], 4);
+        if (!aligned) return fail(CBX_ERR_INVALID_ARG, "%s: an argument is not aligned to its type", name);
         for (int i = 0; i < 9; ++i) {
             for (int j = 0; j < 6; ++j)
                 if (!(i == j && i < 4 && out[i] == in[j]) && overlaps(out[i], no[i], in[j], ni[j]))

@@ -249,3 +249,49 @@ def test_wrappers_run_with_their_tensors_device_current(monkeypatch):
         with pytest.raises(ValueError):
             fn(**kw)
     assert len(calls) == 12
+
+
+def at(addr):
+    return ctypes.c_void_p(addr)
+
+
+def test_misaligned_arguments_are_refused(lib):
+    """Every pointer of the paged entry points and of cbx_token_logprobs, two bytes (one for 16-bit data) off
+    its type's boundary: refused before a launch."""
+    for name in ("lens", "new", "ti", "bi", "fi", "ni", "to", "bo", "fo", "no", "slots", "pos", "reqs", "rl", "start", "err"):
+        assert lib.cbx_paged_plan(*plan_args(**{name: at(0x2000002)})) == -1
+        assert "aligned" in lib.cbx_last_error().decode(), name
+    for name, t, ct, off in (("qkv", 0, 0, 2), ("qkv", 1, 0, 1), ("q", 0, 0, 2), ("q", 1, 0, 1), ("ck", 0, 0, 2),
+                             ("cv", 0, 1, 1), ("bias", 0, 0, 2), ("slots", 0, 0, 2), ("err", 0, 0, 2)):
+        assert lib.cbx_qkv_kv_append_paged(*append_args(**{name: at(0x2000000 + off), "t": t, "ct": ct})) == -1
+        assert "aligned" in lib.cbx_last_error().decode(), name
+    for name, qt, off in (("q", 0, 2), ("q", 1, 1), ("out", 0, 2), ("out", 1, 1), ("table", 0, 2), ("rr", 0, 2),
+                          ("lens", 0, 2), ("lse", 0, 2), ("err", 0, 2)):
+        assert lib.cbx_paged_decode_attention(*attn_args(**{name: at(0x2000000 + off), "qt": qt})) == -1
+        assert "aligned" in lib.cbx_last_error().decode(), name
+    good = [P(1), 0, 0, 2, 80, P(2), 4, P(3), P(4), P(5), P(6), P(7), None]
+    for i in (0, 5, 7, 8, 9, 10, 11):
+        assert lib.cbx_token_logprobs(*good[:i], at(0x2000002), *good[i + 1:]) == -1
+        assert "aligned" in lib.cbx_last_error().decode(), i
+
+
+def test_outputs_over_their_inputs_are_refused(lib):
+    """Heads and rows are worked on side by side: attention cannot write over q, nor the epilogue its q over
+    qkv.  Two rows of 4 x 64 f32 at 0x100000; a row of gap behind each is free."""
+    row = 4 * 64 * 4
+    for off in (0, 4, row, 2 * row - 4, 4 - 2 * row):
+        assert lib.cbx_paged_decode_attention(*attn_args(out=at(0x100000 + off))) == -1
+        assert "overlaps q" in lib.cbx_last_error().decode(), off
+    assert lib.cbx_paged_decode_attention(*attn_args(lse=at(0x100000 + 64))) == -1
+    assert "overlaps q" in lib.cbx_last_error().decode()
+    wide = dict(qs=4 * 256)  # rows four rows apart
+    for off in (4 - 2 * row, 0, 3 * row - 4, 2 * row + 4, 4 * row, 5 * row - 4):
+        assert lib.cbx_paged_decode_attention(*attn_args(out=at(0x100000 + off), **wide)) == -1
+        assert "overlaps q" in lib.cbx_last_error().decode(), off
+    # where they do not meet, the next check answers (the caches' alignment)
+    for off in (-2 * row, row, 2 * row, 5 * row):
+        assert lib.cbx_paged_decode_attention(*attn_args(out=at(0x100000 + off), ck=at(0x200008), **wide)) == -1
+        assert "16-byte" in lib.cbx_last_error().decode(), off
+    for off in (0, 512, 2 * 512 - 4, 4 - 2 * 64 * 4):  # two rows of 128 f32, q of 64
+        assert lib.cbx_qkv_kv_append_paged(*append_args(q=at(0x100000 + off))) == -1
+        assert "overlaps qkv" in lib.cbx_last_error().decode(), off
