@@ -357,6 +357,11 @@ inline Tensor* qkv_kv_append(const Tensor& qkv, const Tensor* qkv_b, Tensor& cac
         ret);
 }
 
+namespace detail {
+// No tensor, or a dense one of 4-byte elements (int32 or f32).
+inline bool dense32(const Tensor* t) { return !t || (type_size(t->type) == 4 && contiguous(*t)); }
+}  // namespace detail
+
 // State of a paged KV cache, all int32 on the device: block_table ne =
 // (max_blocks, n_reqs), n_blocks ne = (n_reqs), free_list ne = (n_pages), n_free
 // ne = (1).  Initially: block_table -1, n_blocks 0, free_list 0 .. n_pages - 1,
@@ -379,6 +384,13 @@ inline Tensor* paged_plan(const Tensor& seq_lens, const Tensor* n_new, PagedStat
         nelements(positions) != rows || (row_reqs && nelements(*row_reqs) != rows) ||
         (row_lens && nelements(*row_lens) != rows)) {
         std::fprintf(stderr, "paged_plan: state and rows of unequal sizes\n");
+        return nullptr;
+    }
+    if (!detail::dense32(&seq_lens) || !detail::dense32(n_new) || !detail::dense32(&st.block_table) ||
+        !detail::dense32(&st.n_blocks) || !detail::dense32(&st.free_list) ||
+        !detail::dense32(&st.n_free) || !detail::dense32(&slots) || !detail::dense32(&positions) ||
+        !detail::dense32(row_reqs) || !detail::dense32(row_lens)) {
+        std::fprintf(stderr, "paged_plan: dense int32 tensors required\n");
         return nullptr;
     }
     return detail::report(
@@ -415,6 +427,7 @@ inline Tensor* qkv_kv_append_paged(const Tensor& qkv, const Tensor* qkv_b, Tenso
     const int64_t kv = cache_k.ne[0], qd = qkv.ne[0] - 2 * kv;
     if (!detail::uniform_rows(qkv, &sx) || !detail::paged_cache(cache_k, cache_v, &ps) || qd < 0 ||
         nelements(slots) < nrows(qkv) || (qkv_b && nelements(*qkv_b) != qkv.ne[0]) ||
+        !detail::dense32(&slots) || !detail::dense32(qkv_b) ||
         (q_out && (q_out->type != qkv.type || !detail::contiguous(*q_out) ||
                    nelements(*q_out) != qd * nrows(qkv)))) {
         std::fprintf(stderr, "qkv_kv_append_paged: rows of q_dim + 2 kv_dim and paged caches of one type\n");
@@ -445,8 +458,10 @@ inline Tensor* paged_decode_attention(const Tensor& q, const Tensor& cache_k, co
     if (!detail::paged_cache(cache_k, cache_v, &ps) || !detail::contiguous(q) ||
         !detail::contiguous(out) || out.type != q.type || nelements(out) != nelements(q) ||
         q.ne[3] != 1 || hd < 1 || cache_k.ne[0] % hd || nelements(seq_lens) != rows ||
-        (row_reqs && nelements(*row_reqs) != rows) || (lse && nelements(*lse) != q.ne[1] * rows)) {
-        std::fprintf(stderr, "paged_decode_attention: q, out and caches of matching sizes\n");
+        (row_reqs && nelements(*row_reqs) != rows) || (lse && nelements(*lse) != q.ne[1] * rows) ||
+        !detail::dense32(&block_table) || !detail::dense32(row_reqs) ||
+        !detail::dense32(&seq_lens) || !detail::dense32(lse)) {
+        std::fprintf(stderr, "paged_decode_attention: q, out and caches of matching sizes, all dense\n");
         return nullptr;
     }
     return detail::report(
@@ -473,8 +488,10 @@ inline Tensor* token_logprobs(const Tensor& logits, const Tensor* tokens, Tensor
     if (!detail::uniform_rows(logits, &sx) || (tokens != nullptr) != (logprob != nullptr) ||
         (tokens && (nelements(*tokens) != n || nelements(*logprob) != n)) ||
         (entropy && nelements(*entropy) != n) || (top_ids != nullptr) != (top_logprobs != nullptr) ||
-        (top_ids && (nrows(*top_ids) != n || nelements(*top_logprobs) != nelements(*top_ids)))) {
-        std::fprintf(stderr, "token_logprobs: rows of logits and outputs of matching sizes\n");
+        (top_ids && (nrows(*top_ids) != n || nelements(*top_logprobs) != nelements(*top_ids))) ||
+        !detail::dense32(tokens) || !detail::dense32(logprob) || !detail::dense32(entropy) ||
+        !detail::dense32(top_ids) || !detail::dense32(top_logprobs)) {
+        std::fprintf(stderr, "token_logprobs: rows of logits and dense outputs of matching sizes\n");
         return nullptr;
     }
     auto f32 = [](Tensor* t) { return t ? static_cast<float*>(t->data) : nullptr; };
