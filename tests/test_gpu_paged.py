@@ -613,3 +613,58 @@ def test_attention_grouped_heads_of_more_than_128_elements(ops, qt, ct, H, Hk, h
         n = a[4][reqs.long()].contiguous()
         got = ops.paged_decode_attention(many, *a[1:4], n, row_reqs=reqs)
         check_attention(got, attention_ref(many, *a[1:4], n, reqs))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 1e-30, 3.0])
+@pytest.mark.parametrize("qt,ct,H,Hk", [(F32, F32, 2, 1), (F32, F32, 8, 2), (F32, F16, 4, 1), (F32, BF16, 8, 2), (F16, F16, 4, 4), (BF16, BF16, 4, 1)])
+def test_attention_of_any_scale(ops, qt, ct, H, Hk, scale):
+    a = make([700, 33, 0, 1], H, Hk, 64, 16, qt, ct, 5)
+    out, lse = ops.paged_decode_attention(*a, scale=scale, return_lse=True)
+    # the reference's bound takes the scale as |scale|: its sign goes to q, which is exact
+    ref = attention_ref(math.copysign(1.0, scale) * a[0], *a[1:], scale=abs(scale))
+    check_attention(out, ref, lse)
+
+
+def test_plan_in_place_with_the_most_requests(ops):
+    B = 8192
+    lens = [(b * 37) % 65 for b in range(B)]
+    st = pool(B, 4, B * 4)
+    p = ops.paged_plan(ints(lens), ints(st["table"]), ints(st["n_blocks"]), ints(st["free"]), ints([B * 4]), 16,
+                       n_new=ints(lens), max_rows=sum(lens), in_place=True)
+    ref = plan_ref(lens, lens, st["table"], st["n_blocks"], st["free"], B * 4, 16, sum(lens))
+    check_plan(p, ref)
+    cut = [n // 2 for n in lens]
+    p = ops.paged_plan(ints(cut), p.block_table, p.n_blocks, p.free_list, p.n_free, 16, n_new=ints([0] * B), max_rows=0,
+                       in_place=True)
+    check_plan(p, plan_ref(cut, [0] * B, ref[5], ref[6], ref[7], ref[8], 16, 0))
+
+
+def test_attention_split_calls_at_the_same_time_and_replayed(ops):
+    """Two captured calls that split a long cache over the workspace, each with its own, replayed on two
+    streams while their lengths change: what the eager calls give."""
+    calls = []
+    for k in range(2):
+        q, ck, cv, table, n = make([30001], 2, 1, 64, 16, F32, BF16, 20 + k)
+        need = ops.paged_decode_attention_workspace(1, 2, 1, 64, table.shape[1], 16, BF16)
+        assert need > 0
+        ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+        args = (q, ck, cv, table, n)
+        ops.paged_decode_attention(*args, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.paged_decode_attention(*args, workspace=ws)
+        calls.append((args, g, out, torch.cuda.Stream()))
+    for lens in ((30001, 30001), (1, 29000), (0, 17), (257, 4096), (30001, 2)):
+        for (args, g, out, s), n in zip(calls, lens):
+            args[4].fill_(n)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for args, g, out, s in calls:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for args, g, out, s in calls:
+            assert torch.equal(out, ops.paged_decode_attention(*args))
+            check_attention(out, attention_ref(*args))
+    del calls
