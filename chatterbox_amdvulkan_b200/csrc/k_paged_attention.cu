@@ -11,14 +11,14 @@
 // end.  Exponentials are base 2 (scale log2 e is folded into q).
 //
 // Bound by HBM: each key and value is read once and takes 2 FMAs per query
-// head.  Two kernels, both with whole tiles of keys and values in flight per
+// head.  Three kernels, all with whole tiles of keys and values in flight per
 // warp and no CTA barrier in the loop:
 //  - k_attend_fma: one query head per kv head, two with an f32 cache, or heads
 //    of more than 128 elements.  A key row of one kv head is VL 16-byte vectors,
 //    one per lane, so a warp reads 32 / VL keys per load instruction.  f32 FMAs.
-//  - k_attend_mma, k_attend_mma_f32: more query heads per kv head, where the
-//    FMAs and the conversions to f32 would bound it.  mma.sync of 16 rows: the
-//    up to 8 query heads of a kv head, twice.
+//  - k_attend_mma (16-bit caches) and k_attend_mma_f32: more query heads per kv
+//    head, where the FMAs and the conversions to f32 would bound it.  mma.sync of
+//    16 rows: the up to 8 query heads of a kv head, twice.
 //
 // The keys of a row are split over the CTAs of a cluster (up to 8), which join
 // their states through distributed shared memory, or, where even that leaves
@@ -1285,7 +1285,7 @@ cudaError_t run_mma_f32(AttnArgs a, int64_t n_rows, cudaStream_t st) {
 template <typename TC>
 cudaError_t run_head(const AttnArgs& a, int cache_type, int64_t n_rows, cudaStream_t st) {
     // Heads of up to 96 elements in rings made for 128: 100 rows of 2000 keys, 32
-    // heads over 8 of 80, f32, 245 us (276 as 128); 3000 keys, f16, 137 (154).
+    // heads over 8 of 80, f32, 239 us (275 as 128); 3000 keys, f16, 143 (152).
     if constexpr (sizeof(TC) == 2) {
         const bool same = a.q_type == cache_type;
         if (use_mma(cache_type, a.group, a.head_dim))

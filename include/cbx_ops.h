@@ -476,8 +476,8 @@ CBX_API int cbx_paged_plan(const int32_t* seq_lens, const int32_t* n_new, int64_
  * q_out may be NULL.  A row with slot -1 is skipped, its q_out row left as it
  * was; any other slot outside [0, n_pages * page_size) writes no cache row and
  * ORs CBX_EFLAG_PAGE_OOB into *err_word (its q_out row is written).  Two rows
- * with one slot leave either's values there.  q_out and the caches must not
- * overlap the inputs. */
+ * with one slot leave either's values there, element by element.  q_out and the
+ * caches must not overlap the inputs; pointers are aligned to their types. */
 CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_row_stride,
                                     const float* qkv_bias, int64_t n_rows, int64_t q_dim,
                                     int64_t kv_dim, const int32_t* slots, void* cache_k,
@@ -497,8 +497,12 @@ CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_r
  * apart (0 = dense; out is dense); caches as in cbx_qkv_kv_append_paged with
  * kv_dim = n_kv_heads * head_dim, of cache_type; table [n_reqs][max_blocks].
  * q_type and cache_type: any of F32 / F16 / BF16.  Products, softmax and sums
- * are f32 (the tensor cores' products of an f32 cache, for 3 and more query
- * heads per kv head, take keys and values to 2^-21); out is rounded once.
+ * are f32, out is rounded once.  Where the tensor cores form the products they
+ * take, of an f32 cache (3 and more query heads per kv head), keys and values to
+ * 2^-21; of a 16-bit cache (2 and more), keys and values as they are, q of
+ * another type to 2^-22 of its largest element (f16) or 2^-24 (bf16), and the
+ * weights e^(s_j - m) of the numerator to 2^-22 (f16), 2^-16 (bf16 with q of
+ * bf16) or 2^-24 (bf16 with another q).
  * Several rows may name one request (the tokens of a prefill chunk or of a
  * speculated continuation, each with its length).  A row of length 0 gives zeros
  * and lse -inf, and so does one whose scores are all -inf.  Infinities and NaN in
@@ -509,9 +513,11 @@ CBX_API int cbx_qkv_kv_append_paged(const void* qkv, int qkv_type, int64_t qkv_r
  * sums and raise CBX_EFLAG_PAGE_OOB, a row_reqs entry outside [0, n_reqs) does
  * too (the row counts as empty); a length above max_blocks * page_size or below
  * 0 is clamped and raises CBX_EFLAG_LENGTH.
- * n_rows * n_heads below 2^31; head_dim: a multiple of 8, at most 256; caches 16-byte aligned, page_stride a
- * multiple of kv_dim and the cache at most 2^31 - 1 rows of kv_dim long
- * (n_pages * page_stride / kv_dim).  out and lse must not overlap the inputs.
+ * n_rows * n_heads below 2^31; head_dim: a multiple of 8, at most 256; caches
+ * 16-byte aligned, everything else aligned to its type; page_stride a multiple
+ * of kv_dim and the cache at most 2^31 - 1 rows of kv_dim long (n_pages *
+ * page_stride / kv_dim).  out and lse must not overlap the inputs (q in place is
+ * refused).
  * workspace: device memory of cbx_paged_decode_attention_workspace(...) bytes,
  * 16-byte aligned, for the partial results of a call that is split over the
  * keys (0 bytes: it may be NULL).  Its contents need no preparation and mean
